@@ -59,6 +59,11 @@ EXPORTED = (
     "g5moe_forward",
     "g5moe_attn_workspace_size",
     "g5moe_attn_varlen_fwd",
+    "g5moe_attn_local_fwd",
+    "g5moe_attn_bwd_workspace_size",
+    "g5moe_attn_bwd",
+    "g5moe_dropout_add",
+    "g5moe_dropout_add_backward",
 )
 
 
@@ -115,6 +120,21 @@ class AttnShape(ctypes.Structure):
     ]
 
 
+class AttnOptions(ctypes.Structure):
+    """Mirror of `g5moe_attn_options`."""
+
+    _fields_ = [
+        ("window_left", ctypes.c_int32),
+        ("window_right", ctypes.c_int32),
+        ("sink_tokens", ctypes.c_int32),
+        ("bias_buckets", ctypes.c_int32),
+        ("bias_distance", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("dropout", Dropout),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class G5MoEError(RuntimeError):
     """A nonzero g5moe_status, with the library's message."""
 
@@ -126,6 +146,8 @@ class G5MoEError(RuntimeError):
 _P = ctypes.c_void_p
 _SHAPE_P = ctypes.POINTER(Shape)
 _DROP_P = ctypes.POINTER(Dropout)
+_ATTN_P = ctypes.POINTER(AttnShape)
+_OPTS_P = ctypes.POINTER(AttnOptions)
 _SIGS = {
     "g5moe_last_error": ([], ctypes.c_char_p),
     "g5moe_version": ([], ctypes.c_int32),
@@ -184,6 +206,16 @@ _SIGS = {
                                   ctypes.c_int),
     "g5moe_attn_varlen_fwd": ([_P, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P,
                                ctypes.POINTER(AttnShape), _P], ctypes.c_int),
+    "g5moe_attn_local_fwd": ([_P] * 8 + [ctypes.c_float, _P, _P, _OPTS_P, _ATTN_P, _P],
+                             ctypes.c_int),
+    "g5moe_attn_bwd_workspace_size": ([_OPTS_P, _ATTN_P, ctypes.POINTER(ctypes.c_size_t)],
+                                      ctypes.c_int),
+    "g5moe_attn_bwd": ([_P] * 10 + [ctypes.c_float] + [_P] * 5 +
+                       [_OPTS_P, _ATTN_P, _ATTN_P, _P], ctypes.c_int),
+    "g5moe_dropout_add": ([_P, _P, _P, _DROP_P, ctypes.c_float, ctypes.c_int64, ctypes.c_int32,
+                           ctypes.c_int32, _P], ctypes.c_int),
+    "g5moe_dropout_add_backward": ([_P, _P, _DROP_P, ctypes.c_float, ctypes.c_int64,
+                                    ctypes.c_int32, ctypes.c_int32, _P], ctypes.c_int),
 }
 
 _lock = threading.Lock()

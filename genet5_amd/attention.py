@@ -1,4 +1,5 @@
-"""Varlen bidirectional ALiBi attention on the HIP kernel of libg5moe.so.
+"""Varlen bidirectional attention on the HIP kernels of libg5moe.so: ALiBi or a learned
+bucketed position bias, a sliding window with sink tokens, dropout, and the backward.
 
 Reference interface: GeneT5's FlashAttention (lib/blocks/_flash_att.py:15-98)
 calls flash-attn's
@@ -15,12 +16,17 @@ sequence-local positions) and a `FlashAttention`-shaped module whose
 `forward(hidden_states, cu_seqlens=None, max_seqlen=None)` returns
 `(out, None)` like the reference's.
 
-Supported: bf16, head_dim 64, non-causal, no dropout, forward only.  Anything
-else raises; there is no CPU or PyTorch fallback.
+Beyond flash-attn's arguments: `sink_tokens` (first tokens of each sequence that stay
+visible outside the window), `relative_bias` with `max_distance` (a learned bias
+[num_buckets, heads] over bucketed relative positions) and `dropout_seed`.
+
+Supported: bf16, head_dim 64, self-attention, forward and backward.  Anything else
+raises; there is no CPU or PyTorch fallback.
 """
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import List, Optional, Tuple
@@ -148,24 +154,363 @@ def _no_backward(ctx, *grads):
 _attn_op.register_autograd(_no_backward)
 
 
-def _unsupported(dropout_p, causal, window_size):
-    if dropout_p:
-        raise NotImplementedError("attention dropout is not supported (dropout_p must be 0)")
+# ---- window, sinks, bucketed position bias, dropout, backward -------------------------
+
+MAX_BIAS_DISTANCE = 1024
+
+
+@functools.lru_cache(maxsize=64)
+def _bucket_starts(num_buckets: int, max_distance: int) -> Tuple[int, ...]:
+    """The smallest distance of each bucket of one side after the first, in whole numbers.
+    Of a side's half = num_buckets / 2 buckets the first e = half / 2 hold one distance
+    each; bucket e + s starts at the smallest n with (n / e)^(half - e) >= (D / e)^s, i.e.
+    log(n / e) / log(D / e) (half - e) >= s without rounding."""
+    half = num_buckets // 2
+    e = half // 2
+    starts = list(range(1, e + 1))
+    for s in range(1, half - e):
+        lo, hi = starts[-1], max_distance
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** (half - e) * e ** s >= max_distance ** s * e ** (half - e):
+                hi = mid
+            else:
+                lo = mid + 1
+        starts.append(lo)
+    return tuple(starts)
+
+
+def _check_buckets(num_buckets: int, max_distance: int) -> None:
+    if num_buckets < 4 or num_buckets % 2:
+        raise ValueError(f"num_buckets {num_buckets} must be even and at least 4 (half of them "
+                         "for keys after the query)")
+    if not num_buckets // 4 < max_distance <= MAX_BIAS_DISTANCE:
+        raise ValueError(f"max_distance {max_distance} must exceed num_buckets / 4 = "
+                         f"{num_buckets // 4} and be at most {MAX_BIAS_DISTANCE}")
+
+
+def relative_buckets(num_buckets: int, max_distance: int,
+                     device: Optional[torch.device] = None) -> torch.Tensor:
+    """int32 [2 * max_distance + 1]: the bucket of each relative position r = key - query
+    from -max_distance to max_distance; positions farther away share the ends' buckets.
+    Keys after the query (r > 0) use the upper half of the buckets.  With half =
+    num_buckets / 2 and e = half / 2, distances below e have a bucket each, distance n >= e
+    is in bucket e + floor(log(n / e) / log(max_distance / e) (half - e)), half - 1 at most
+    (exact at the borders, whatever a logarithm rounds to)."""
+    _check_buckets(num_buckets, max_distance)
+    starts = torch.tensor(_bucket_starts(num_buckets, max_distance))
+    n = torch.arange(max_distance + 1)
+    side = torch.searchsorted(starts, n, right=True)
+    out = torch.cat([side.flip(0), side[1:] + num_buckets // 2])
+    return out.to(torch.int32).to(device) if device is not None else out.to(torch.int32)
+
+
+_BUCKETS: dict = {}
+
+
+def _buckets_on(num_buckets: int, max_distance: int, device: torch.device) -> torch.Tensor:
+    """relative_buckets on `device`, built once per device and pair of numbers."""
+    key = (num_buckets, max_distance, device)
+    t = _BUCKETS.get(key)
+    if t is None:
+        if len(_BUCKETS) >= 64:
+            _BUCKETS.clear()
+        t = _BUCKETS[key] = relative_buckets(num_buckets, max_distance, device)
+        if device.type == "cuda" and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()  # used on any stream from now on
+    return t
+
+
+def _check_cu(cu_seqlens: torch.Tensor, dev: torch.device) -> None:
+    if cu_seqlens.device != dev or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 \
+            or cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
+        raise ValueError("cu_seqlens must be a contiguous int32 vector [n_seqs + 1] on "
+                         f"{dev}")
+
+
+def _options(window_left: int, window_right: int, sink_tokens: int, dropout_p: float, seed: int,
+             bias: Optional[torch.Tensor], max_distance: int) -> _lib.AttnOptions:
+    o = _lib.AttnOptions(window_left, window_right, sink_tokens, 0, 0, 0,
+                         _lib.make_dropout(dropout_p, seed), 0)
+    if bias is not None:
+        o.bias_buckets = bias.shape[0]
+        o.bias_distance = max_distance
+        o.bias_dtype = ops._dtype_code(bias.dtype)
+    return o
+
+
+def _check_position(alibi_slopes: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                    max_distance: int, H: int, dev: torch.device) -> None:
+    if alibi_slopes is not None:
+        if alibi_slopes.device != dev or alibi_slopes.dtype != torch.float32 \
+                or tuple(alibi_slopes.shape) != (H,) or not alibi_slopes.is_contiguous():
+            raise ValueError(f"alibi_slopes must be a contiguous float32 [{H}] tensor on {dev}")
+        if bias is not None:
+            raise ValueError("alibi_slopes and relative_bias exclude each other")
+    if bias is not None:
+        if bias.device != dev:
+            raise ValueError(f"relative_bias is on {bias.device}, expected {dev}")
+        if bias.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"relative_bias has dtype {bias.dtype}; it must be bfloat16 or "
+                            "float32")
+        if bias.dim() != 2 or bias.shape[1] != H:
+            raise ValueError(f"relative_bias has shape {tuple(bias.shape)}, expected "
+                             f"(num_buckets, {H})")
+        _check_buckets(bias.shape[0], max_distance)
+
+
+def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                   max_seqlen: int, softmax_scale: float,
+                   alibi_slopes: Optional[torch.Tensor] = None,
+                   relative_bias: Optional[torch.Tensor] = None, max_distance: int = 128,
+                   window_size: Tuple[int, int] = (-1, -1), sink_tokens: int = 0,
+                   dropout_p: float = 0.0, dropout_seed: int = 0, return_lse: bool = False):
+    """g5moe_attn_local_fwd on the current stream: attention over the visible keys with an
+    optional position bias and dropout.  Tensors as attn_varlen_fwd takes them;
+    relative_bias [num_buckets, H] bf16 or fp32.  Returns out [T, H, 64] (and softmax_lse
+    [H, T] fp32 when return_lse); rows behind the last sequence are zeros in out."""
+    dev = _check_device(q)
+    T, H = q.shape[0], q.shape[1]
+    Hkv = k.shape[1] if k.dim() == 3 else -1
+    _check_qkv(q, "q", T, H, dev)
+    _check_qkv(k, "k", T, Hkv, dev)
+    _check_qkv(v, "v", T, Hkv, dev)
+    if H % Hkv:
+        raise ValueError(f"key/value heads {Hkv} must divide query heads {H}")
+    _check_cu(cu_seqlens, dev)
+    _check_position(alibi_slopes, relative_bias, max_distance, H, dev)
+    bias = None if relative_bias is None else relative_bias.contiguous()
+    buckets = None if bias is None else _buckets_on(bias.shape[0], max_distance, dev)
+    n_seqs, max_seqlen = cu_seqlens.numel() - 1, int(max_seqlen)
+    empty = n_seqs == 0 or max_seqlen <= 0   # nothing is launched
+    out = (torch.zeros if empty else torch.empty)((T + ops.ROW_PAD, H, HEAD_DIM),
+                                                  dtype=torch.bfloat16, device=dev)[:T]
+    lse = torch.empty((H, T), dtype=torch.float32, device=dev) if return_lse else None
+    shape = _lib.AttnShape(n_seqs, max_seqlen, T, H, Hkv, HEAD_DIM, 0, q.stride(0), q.stride(1),
+                           k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
+                           out.stride(1))
+    opts = _options(*window_size, sink_tokens, dropout_p, dropout_seed, bias, max_distance)
+    ws = None
+    if tuple(window_size) == (-1, -1) and bias is None and dropout_p == 0:
+        # the full attention's kernel, with its key-norm bounds
+        ws = torch.empty(_lib.attn_workspace_size(T, H, Hkv, HEAD_DIM), dtype=torch.uint8,
+                         device=dev)
+    ops._call_on(dev, "g5moe_attn_local_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                 _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias), _ptr(buckets),
+                 ctypes.c_float(softmax_scale), _ptr(lse), _ptr(ws), ctypes.byref(opts),
+                 ctypes.byref(shape), _stream(dev))
+    return (out, lse) if return_lse else out
+
+
+def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+             out: torch.Tensor, softmax_lse: torch.Tensor, cu_seqlens: torch.Tensor,
+             max_seqlen: int, softmax_scale: float,
+             alibi_slopes: Optional[torch.Tensor] = None,
+             relative_bias: Optional[torch.Tensor] = None, max_distance: int = 128,
+             window_size: Tuple[int, int] = (-1, -1), sink_tokens: int = 0,
+             dropout_p: float = 0.0, dropout_seed: int = 0, bias_grad: bool = True):
+    """g5moe_attn_bwd on the current stream: (dq, dk, dv, d_relative_bias) of a forward with
+    these arguments, from its out and softmax_lse; d_relative_bias is None without a table
+    or with bias_grad = False.  Rows behind the last sequence are zeros."""
+    dev = _check_device(q)
+    T, H = q.shape[0], q.shape[1]
+    Hkv = k.shape[1] if k.dim() == 3 else -1
+    _check_qkv(q, "q", T, H, dev)
+    _check_qkv(k, "k", T, Hkv, dev)
+    _check_qkv(v, "v", T, Hkv, dev)
+    _check_qkv(out, "out", T, H, dev)
+    _check_qkv(dout, "dout", T, H, dev)
+    if H % Hkv:
+        raise ValueError(f"key/value heads {Hkv} must divide query heads {H}")
+    _check_cu(cu_seqlens, dev)
+    _check_position(alibi_slopes, relative_bias, max_distance, H, dev)
+    ops._require(softmax_lse, "softmax_lse", (H, T), torch.float32, dev)
+    bias = None if relative_bias is None else relative_bias.contiguous()
+    buckets = None if bias is None else _buckets_on(bias.shape[0], max_distance, dev)
+    n_seqs, max_seqlen = cu_seqlens.numel() - 1, int(max_seqlen)
+    empty = n_seqs == 0 or max_seqlen <= 0 or T == 0   # nothing is launched
+    new = torch.zeros if empty else torch.empty
+    dq, dk, dv = (new((T, h, HEAD_DIM), dtype=torch.bfloat16, device=dev) for h in (H, Hkv, Hkv))
+    dbias = None
+    if bias is not None and bias_grad:
+        dbias = (torch.zeros_like if empty else torch.empty_like)(bias)
+    if empty:
+        return dq, dk, dv, dbias
+    sizes = (n_seqs, max_seqlen, T, H, Hkv, HEAD_DIM, 0)
+    shape = _lib.AttnShape(*sizes, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                           v.stride(0), v.stride(1), out.stride(0), out.stride(1))
+    gshape = _lib.AttnShape(*sizes, dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1),
+                            dv.stride(0), dv.stride(1), dout.stride(0), dout.stride(1))
+    opts = _options(*window_size, sink_tokens, dropout_p, dropout_seed, bias, max_distance)
+    n = ctypes.c_size_t(0)
+    _lib.call("g5moe_attn_bwd_workspace_size", ctypes.byref(opts), ctypes.byref(shape),
+              ctypes.byref(n))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    ops._call_on(dev, "g5moe_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                 _ptr(softmax_lse), _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias),
+                 _ptr(buckets), ctypes.c_float(softmax_scale), _ptr(dq), _ptr(dk), _ptr(dv),
+                 _ptr(dbias), _ptr(ws), ctypes.byref(opts), ctypes.byref(shape),
+                 ctypes.byref(gshape), _stream(dev))
+    return dq, dk, dv, dbias
+
+
+def _draw_seed() -> int:
+    """A dropout seed from torch's default CPU generator (torch.manual_seed reproduces it)."""
+    return int(torch.randint(0, 2 ** 62, (1,)).item())
+
+
+def _bwd_call(need_bias, dout, q, k, v, out, lse, cu, slopes, bias, call, seed):
+    """attn_bwd with dout brought into a form the kernel reads."""
+    max_seqlen, scale, max_distance, wl, wr, sinks, p = call
+    st = dout.stride()
+    if dout.dtype != torch.bfloat16 or st[2] != 1 or st[0] % 8 or st[1] % 8 \
+            or dout.data_ptr() % 16:
+        dout = dout.to(torch.bfloat16).contiguous()
+    return attn_bwd(dout, q, k, v, out, lse, cu, max_seqlen, scale, slopes, bias, max_distance,
+                    (wl, wr), sinks, p, seed, need_bias)
+
+
+class _AttnFunction(torch.autograd.Function):
+    """The differentiable attention of eager programs (a traced one records the custom op
+    below, whose dispatch costs more host time per call)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, cu, max_seqlen, scale, slopes, max_distance, wl, wr, sinks,
+                p, seed):
+        out, lse = attn_local_fwd(q, k, v, cu, max_seqlen, scale, slopes, bias, max_distance,
+                                  (wl, wr), sinks, p, seed, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu, slopes, bias)
+        ctx.call = (max_seqlen, scale, max_distance, wl, wr, sinks, p)
+        ctx.seed = seed
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        none = (None,) * 14
+        if dout is None:
+            return none
+        need = ctx.needs_input_grad
+        grads = _bwd_call(need[3], dout, *ctx.saved_tensors, ctx.call, ctx.seed)
+        return tuple(g if n else None for g, n in zip(grads, need)) + none[4:]
+
+
+@torch.library.custom_op("g5moe::attn_local", mutates_args=())
+def _attn_local_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                   max_seqlen: int, softmax_scale: float, alibi_slopes: Optional[torch.Tensor],
+                   relative_bias: Optional[torch.Tensor], max_distance: int, window_left: int,
+                   window_right: int, sink_tokens: int, dropout_p: float,
+                   dropout_seed: Optional[int]
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(out, softmax_lse [H, T], the dropout seed as host int64 [1]).  With dropout and no
+    seed the op draws one per call, so a compiled program draws anew each time."""
+    seed = 0
+    if dropout_p > 0:
+        seed = _draw_seed() if dropout_seed is None else dropout_seed
+    out, lse = attn_local_fwd(q, k, v, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes,
+                              relative_bias, max_distance, (window_left, window_right),
+                              sink_tokens, dropout_p, seed, return_lse=True)
+    return out, lse, torch.tensor([seed], dtype=torch.int64)
+
+
+@_attn_local_op.register_fake
+def _(q, k, v, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes, relative_bias, max_distance,
+      window_left, window_right, sink_tokens, dropout_p, dropout_seed):
+    T, H, D = q.shape
+    return (q.new_empty((T, H, D)), q.new_empty((H, T), dtype=torch.float32),
+            torch.empty((1,), dtype=torch.int64, device="cpu"))
+
+
+@torch.library.custom_op("g5moe::attn_local_backward", mutates_args=())
+def _attn_local_bwd_op(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       out: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
+                       max_seqlen: int, softmax_scale: float,
+                       alibi_slopes: Optional[torch.Tensor],
+                       relative_bias: Optional[torch.Tensor], max_distance: int,
+                       window_left: int, window_right: int, sink_tokens: int, dropout_p: float,
+                       seed: torch.Tensor, bias_grad: bool
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv, d_relative_bias or an empty tensor)."""
+    dq, dk, dv, db = _bwd_call(bias_grad, dout, q, k, v, out, lse, cu_seqlens, alibi_slopes,
+                               relative_bias, (max_seqlen, softmax_scale, max_distance,
+                                               window_left, window_right, sink_tokens,
+                                               dropout_p), int(seed[0]))
+    return dq, dk, dv, q.new_empty((0,)) if db is None else db
+
+
+@_attn_local_bwd_op.register_fake
+def _(dout, q, k, v, out, lse, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes,
+      relative_bias, max_distance, window_left, window_right, sink_tokens, dropout_p, seed,
+      bias_grad):
+    grads = tuple(t.new_empty(t.shape) for t in (q, k, v))
+    if relative_bias is None or not bias_grad:
+        return grads + (q.new_empty((0,)),)
+    return grads + (relative_bias.new_empty(relative_bias.shape),)
+
+
+def _local_setup(ctx, inputs, output):
+    (q, k, v, cu, max_seqlen, scale, slopes, bias, max_distance, wl, wr, sinks, p, _) = inputs
+    out, lse, seed = output
+    ctx.save_for_backward(q, k, v, out, lse, cu, slopes, bias, seed)
+    ctx.call = (max_seqlen, scale, max_distance, wl, wr, sinks, p)
+    ctx.mark_non_differentiable(lse, seed)
+    ctx.set_materialize_grads(False)
+
+
+def _local_backward(ctx, dout, _dlse, _dseed):
+    grads = [None] * 14
+    if dout is not None:
+        q, k, v, out, lse, cu, slopes, bias, seed = ctx.saved_tensors
+        max_seqlen, scale, max_distance, wl, wr, sinks, p = ctx.call
+        need = ctx.needs_input_grad
+        dq, dk, dv, db = _attn_local_bwd_op(dout, q, k, v, out, lse, cu, max_seqlen, scale,
+                                            slopes, bias, max_distance, wl, wr, sinks, p, seed,
+                                            need[7])
+        for i, g in ((0, dq), (1, dk), (2, dv), (7, db)):
+            if need[i]:
+                grads[i] = g
+    return tuple(grads)
+
+
+_attn_local_op.register_autograd(_local_backward, setup_context=_local_setup)
+
+
+def _unsupported(causal, window_size):
     if causal:
         raise NotImplementedError("causal attention is not supported (GeneT5's encoder is "
-                                  "bidirectional)")
-    if tuple(window_size) != (-1, -1):
-        raise NotImplementedError("local (windowed) attention is not supported")
+                                  "bidirectional); window_size=(-1, 0) leaves out the keys "
+                                  "after each query")
+    if len(tuple(window_size)) != 2 or any(int(w) != w or w < -1 for w in window_size):
+        raise ValueError(f"window_size {window_size!r} must be two integers >= -1 (-1: no limit "
+                         "on that side)")
 
 
 def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                            dropout_p=0.0, softmax_scale=None, causal=False,
                            window_size=(-1, -1), alibi_slopes=None, deterministic=False,
-                           return_attn_probs=False):
-    """flash-attn's varlen entry point over the HIP kernel (self-attention: the
+                           return_attn_probs=False, *, sink_tokens=0, relative_bias=None,
+                           max_distance=128, dropout_seed=None):
+    """flash-attn's varlen entry point over the HIP kernels (self-attention: the
     query and key segmentations must be the same).  Returns out [T, H, D], or
-    (out, softmax_lse, None) with return_attn_probs."""
-    _unsupported(dropout_p, causal, window_size)
+    (out, softmax_lse, None) with return_attn_probs.  Differentiable in q, k, v and
+    relative_bias; every result is deterministic.
+
+    window_size (left, right): query i sees the keys i - left .. i + right of its sequence
+    (-1: no limit), and with sink_tokens = n its first n tokens always.  relative_bias
+    [num_buckets, H] (bf16 or fp32) is added to the scaled scores by the bucket of
+    key - query (relative_buckets); it excludes alibi_slopes.  dropout_p drops
+    probabilities after the softmax by the counter-based mask of g5moe_dropout; without
+    dropout_seed (a non-negative integer below 2^63) the 64-bit seed is drawn from torch's
+    CPU generator, one per call (fixed at capture in a HIP graph)."""
+    _unsupported(causal, window_size)
+    if not 0.0 <= dropout_p <= 1.0:
+        raise ValueError(f"dropout_p {dropout_p} is not in [0, 1]")
+    if sink_tokens < 0:
+        raise ValueError(f"sink_tokens {sink_tokens} must be >= 0")
+    if dropout_seed is not None and not 0 <= int(dropout_seed) < 2 ** 63:
+        raise ValueError(f"dropout_seed {dropout_seed} is not in [0, 2^63)")
     if cu_seqlens_k is not cu_seqlens_q and not torch.equal(cu_seqlens_k, cu_seqlens_q):
         raise NotImplementedError("cu_seqlens_k must equal cu_seqlens_q (self-attention)")
     if max_seqlen_q is None:
@@ -175,11 +520,36 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
         raise NotImplementedError("max_seqlen_k must equal max_seqlen_q (self-attention)")
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** -0.5
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-        raise NotImplementedError("the HIP attention kernel is forward-only; call it under "
-                                  "torch.no_grad()")
-    out, lse = _attn_op(q, k, v, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale),
-                        alibi_slopes, bool(return_attn_probs))
+    if dropout_p and q.device.type != "cuda":
+        raise NotImplementedError("attention dropout runs on the GPU only (dropout_p must be 0 "
+                                  f"on {q.device})")
+    wl, wr = (int(w) for w in window_size)
+    leaves = (q, k, v) if relative_bias is None else (q, k, v, relative_bias)
+    grad = torch.is_grad_enabled() and any(t.requires_grad for t in leaves)
+    lse = None
+    if not grad and wl < 0 and wr < 0 and relative_bias is None and dropout_p == 0:
+        out, lse = _attn_op(q, k, v, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale),
+                            alibi_slopes, bool(return_attn_probs))
+    elif torch.compiler.is_compiling():
+        out, lse, _ = _attn_local_op(
+            q, k, v, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale), alibi_slopes,
+            relative_bias, int(max_distance), wl, wr, int(sink_tokens), float(dropout_p),
+            None if dropout_seed is None else int(dropout_seed))
+    else:
+        seed = 0
+        if dropout_p > 0:
+            seed = _draw_seed() if dropout_seed is None else int(dropout_seed)
+        if grad:
+            out, lse = _AttnFunction.apply(
+                q, k, v, relative_bias, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale),
+                alibi_slopes, int(max_distance), wl, wr, int(sink_tokens), float(dropout_p), seed)
+        else:
+            out = attn_local_fwd(
+                q, k, v, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale), alibi_slopes,
+                relative_bias, int(max_distance), (wl, wr), int(sink_tokens), float(dropout_p),
+                seed, return_lse=bool(return_attn_probs))
+            if return_attn_probs:
+                out, lse = out
     return (out, lse, None) if return_attn_probs else out
 
 
@@ -198,15 +568,18 @@ def _uniform_cu_seqlens(batch: int, seqlen: int, device: torch.device) -> torch.
 
 def flash_attn_func(q, k, v, dropout_p=0.0, softmax_scale=None, causal=False,
                     window_size=(-1, -1), alibi_slopes=None, deterministic=False,
-                    return_attn_probs=False):
-    """flash-attn's fixed-length entry point: q [B, L, H, D], k/v [B, L, Hkv, D]."""
-    _unsupported(dropout_p, causal, window_size)
+                    return_attn_probs=False, *, sink_tokens=0, relative_bias=None,
+                    max_distance=128, dropout_seed=None):
+    """flash-attn's fixed-length entry point: q [B, L, H, D], k/v [B, L, Hkv, D]; the other
+    arguments as in flash_attn_varlen_func."""
     B, L = q.shape[0], q.shape[1]
     cu = _uniform_cu_seqlens(B, L, q.device)
     res = flash_attn_varlen_func(q.reshape(B * L, *q.shape[2:]), k.reshape(B * L, *k.shape[2:]),
-                                 v.reshape(B * L, *v.shape[2:]), cu, cu, L, L, 0.0,
-                                 softmax_scale, False, (-1, -1), alibi_slopes, deterministic,
-                                 return_attn_probs)
+                                 v.reshape(B * L, *v.shape[2:]), cu, cu, L, L, dropout_p,
+                                 softmax_scale, causal, window_size, alibi_slopes, deterministic,
+                                 return_attn_probs, sink_tokens=sink_tokens,
+                                 relative_bias=relative_bias, max_distance=max_distance,
+                                 dropout_seed=dropout_seed)
     if return_attn_probs:
         out, lse, _ = res
         return out.view(B, L, *out.shape[1:]), lse, None

@@ -35,7 +35,8 @@ FLAGS = [
     f"-I{INCLUDE_DIR}",
 ]
 SOURCES = ["api.hip", "router.hip", "dispatch.hip", "grouped_gemm.hip", "combine.hip",
-           "backward.hip", "attention.hip", "wgrad.hip", "xcd_balance.hip"]
+           "backward.hip", "attention.hip", "attention_local.hip", "attention_bwd.hip",
+           "dropout_add.hip", "wgrad.hip", "xcd_balance.hip"]
 
 
 def _compile(src: Path, obj: Path, verbose: bool) -> None:

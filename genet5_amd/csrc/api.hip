@@ -3,6 +3,9 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
+
+#include "attn_tile.h"
 #include "g5moe_internal.h"
 
 using namespace g5moe;
@@ -104,7 +107,7 @@ extern "C" {
 
 const char* g5moe_last_error(void) { return g_err; }
 
-int32_t g5moe_version(void) { return (2 << 16) | 3; }
+int32_t g5moe_version(void) { return (2 << 16) | 4; }
 
 g5moe_status g5moe_workspace_size(const g5moe_shape* shape, size_t* bytes) {
   G5_CHECK(check_shape(shape));
@@ -868,6 +871,256 @@ g5moe_status g5moe_attn_varlen_fwd(const void* q, const void* k, const void* v, 
                                     cu_seqlens, alibi_slopes, softmax_scale, softmax_lse,
                                     static_cast<float*>(ws), s, as_stream(stream)),
                     "g5moe_attn_varlen_fwd");
+}
+
+// What the forward and the backward with options check and fill alike.
+static g5moe_status local_args(attn::LocalArgs* a, const int32_t* cu_seqlens,
+                               const float* alibi_slopes, const void* bias_table,
+                               const int32_t* bucket_of, float softmax_scale,
+                               const g5moe_attn_options* options, const g5moe_attn_shape& s) {
+  if (!(softmax_scale == softmax_scale) || softmax_scale == __builtin_inff() ||
+      softmax_scale == -__builtin_inff())
+    return fail(G5MOE_ERR_INVALID_ARG, "softmax_scale must be finite");
+  g5moe_attn_options o{};
+  if (options != nullptr)
+    o = *options;
+  else
+    o.window_left = o.window_right = -1;
+  if (o.reserved != 0) return fail(G5MOE_ERR_INVALID_ARG, "attn options.reserved must be 0");
+  if (o.window_left < -1 || o.window_right < -1 || o.sink_tokens < 0)
+    return fail(G5MOE_ERR_INVALID_ARG,
+                "window_left and window_right must be >= -1 and sink_tokens >= 0 (%d, %d, %d)",
+                int(o.window_left), int(o.window_right), int(o.sink_tokens));
+  *a = attn::LocalArgs{};
+  G5_CHECK(dropout_params(&o.dropout, &a->drop));
+  if (bias_table != nullptr) {
+    G5_NONNULL(bucket_of);
+    if (alibi_slopes != nullptr)
+      return fail(G5MOE_ERR_INVALID_ARG, "alibi_slopes and bias_table exclude each other");
+    if (o.bias_buckets < 1 || o.bias_distance < 1)
+      return fail(G5MOE_ERR_INVALID_ARG, "bias_buckets %d and bias_distance %d must be >= 1",
+                  int(o.bias_buckets), int(o.bias_distance));
+    if (o.bias_distance > G5MOE_MAX_BIAS_DISTANCE)
+      return fail(G5MOE_ERR_UNSUPPORTED, "bias_distance %d exceeds %d", int(o.bias_distance),
+                  G5MOE_MAX_BIAS_DISTANCE);
+    if (o.bias_dtype != G5MOE_DTYPE_BF16 && o.bias_dtype != G5MOE_DTYPE_F32)
+      return fail(G5MOE_ERR_INVALID_ARG, "bias_dtype %d is neither bf16 (0) nor f32 (1)",
+                  int(o.bias_dtype));
+  }
+  // beyond every position: unlimited
+  const int all = int(s.total_tokens);
+  a->wl = o.window_left < 0 ? all : std::min(int(o.window_left), all);
+  a->wr = o.window_right < 0 ? all : std::min(int(o.window_right), all);
+  a->ns = std::min(int(o.sink_tokens), all);
+  a->cu = cu_seqlens;
+  a->n_seqs = s.n_seqs;
+  a->n_heads = s.n_heads;
+  a->group = s.n_heads / s.n_kv_heads;
+  a->scale = softmax_scale;
+  a->sc = softmax_scale * attn::kLog2e;
+  a->slopes = alibi_slopes;
+  a->bias = bias_table;
+  a->bucket_of = bucket_of;
+  a->bias_bf16 = o.bias_dtype == G5MOE_DTYPE_BF16;
+  a->n_buckets = o.bias_buckets;
+  a->far = o.bias_distance;
+  a->total = s.total_tokens;
+  a->max_len = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
+  a->q_tok = s.q_token_stride;
+  a->k_tok = s.k_token_stride;
+  a->v_tok = s.v_token_stride;
+  a->o_tok = s.o_token_stride;
+  a->q_head = s.q_head_stride;
+  a->k_head = s.k_head_stride;
+  a->v_head = s.v_head_stride;
+  a->o_head = s.o_head_stride;
+  return G5MOE_OK;
+}
+
+g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
+                                  const int32_t* cu_seqlens, const float* alibi_slopes,
+                                  const void* bias_table, const int32_t* bucket_of,
+                                  float softmax_scale, float* softmax_lse, void* ws,
+                                  const g5moe_attn_options* options,
+                                  const g5moe_attn_shape* shape, void* stream) {
+  G5_CHECK(check_attn_shape(shape));
+  const g5moe_attn_shape& s = *shape;
+  attn::LocalArgs a;
+  G5_CHECK(local_args(&a, cu_seqlens, alibi_slopes, bias_table, bucket_of, softmax_scale, options,
+                      s));
+  if (s.n_seqs == 0 || s.max_seqlen == 0 || s.total_tokens == 0) return G5MOE_OK;
+  G5_NONNULL(q);
+  G5_NONNULL(k);
+  G5_NONNULL(v);
+  G5_NONNULL(out);
+  G5_NONNULL(cu_seqlens);
+  const uintptr_t align = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                          reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out);
+  if (align % 16 != 0)
+    return fail(G5MOE_ERR_UNSUPPORTED, "q, k, v and out must be 16-byte aligned");
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.o = static_cast<uint16_t*>(out);
+  a.lse = softmax_lse;
+  const bool full =
+      options == nullptr || (options->window_left < 0 && options->window_right < 0);
+  if (full && bias_table == nullptr && !a.drop.on) {
+    // no option is in use: the full attention's kernel
+    g5moe_attn_shape f = s;
+    f.max_seqlen = a.max_len;
+    const hipError_t e = launch_attn_fwd(a.q, a.k, a.v, a.o, cu_seqlens, alibi_slopes,
+                                         softmax_scale, softmax_lse, static_cast<float*>(ws), f,
+                                         as_stream(stream));
+    return hip_status(e != hipSuccess ? e : attn::launch_zero_behind(a, as_stream(stream)),
+                      "g5moe_attn_local_fwd");
+  }
+  const bool wide = std::max(s.k_token_stride, s.v_token_stride) >= (int64_t(1) << 24);
+  return hip_status(attn::launch_local_fwd(a, wide, as_stream(stream)),
+                    "g5moe_attn_local_fwd");
+}
+
+namespace {
+// The backward's workspace: -lse, delta and the dropout row keys per (head, token), the bias
+// sums per workgroup and per distance.
+struct AttnBwdLayout {
+  size_t nl, delta, rowkey, part, rel, total;
+};
+AttnBwdLayout attn_bwd_layout(const g5moe_attn_options* o, const g5moe_attn_shape& s) {
+  AttnBwdLayout w;
+  const size_t rows = align256(size_t(s.n_heads) * size_t(s.total_tokens) * 4);
+  size_t off = 0;
+  w.nl = off;
+  off += rows;
+  w.delta = off;
+  off += rows;
+  w.rowkey = off;
+  if (o != nullptr && o->dropout.p > 0.0f) off += rows;
+  w.part = w.rel = off;
+  if (o != nullptr && o->bias_buckets > 0 && o->bias_distance > 0) {
+    const int top = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
+    off += align256(size_t(attn::bwd_part_floats(top, s.n_seqs, s.n_heads, o->bias_distance)) * 4);
+    w.rel = off;
+    off += align256(size_t(s.n_heads) * size_t(2 * o->bias_distance + 1) * 4);
+  }
+  w.total = off;
+  return w;
+}
+}  // namespace
+
+g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
+                                           const g5moe_attn_shape* shape, size_t* bytes) {
+  G5_CHECK(check_attn_shape(shape));
+  G5_NONNULL(bytes);
+  if (options != nullptr && options->bias_distance > G5MOE_MAX_BIAS_DISTANCE)
+    return fail(G5MOE_ERR_UNSUPPORTED, "bias_distance %d exceeds %d", int(options->bias_distance),
+                G5MOE_MAX_BIAS_DISTANCE);
+  *bytes = attn_bwd_layout(options, *shape).total;
+  return G5MOE_OK;
+}
+
+g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                            const void* out, const float* softmax_lse, const int32_t* cu_seqlens,
+                            const float* alibi_slopes, const void* bias_table,
+                            const int32_t* bucket_of, float softmax_scale, void* dq, void* dk,
+                            void* dv, void* dbias, void* ws, const g5moe_attn_options* options,
+                            const g5moe_attn_shape* shape, const g5moe_attn_shape* grad_shape,
+                            void* stream) {
+  G5_CHECK(check_attn_shape(shape));
+  G5_CHECK(check_attn_shape(grad_shape));
+  const g5moe_attn_shape& s = *shape;
+  const g5moe_attn_shape& g = *grad_shape;
+  if (g.n_seqs != s.n_seqs || g.max_seqlen != s.max_seqlen || g.total_tokens != s.total_tokens ||
+      g.n_heads != s.n_heads || g.n_kv_heads != s.n_kv_heads)
+    return fail(G5MOE_ERR_INVALID_ARG, "grad_shape and shape differ in more than their strides");
+  attn::LocalArgs a;
+  G5_CHECK(local_args(&a, cu_seqlens, alibi_slopes, bias_table, bucket_of, softmax_scale, options,
+                      s));
+  if (dbias != nullptr && bias_table == nullptr)
+    return fail(G5MOE_ERR_INVALID_ARG, "dbias without a bias_table");
+  if (s.n_seqs == 0 || s.max_seqlen == 0 || s.total_tokens == 0) return G5MOE_OK;
+  G5_NONNULL(dout);
+  G5_NONNULL(q);
+  G5_NONNULL(k);
+  G5_NONNULL(v);
+  G5_NONNULL(out);
+  G5_NONNULL(softmax_lse);
+  G5_NONNULL(cu_seqlens);
+  G5_NONNULL(dq);
+  G5_NONNULL(dk);
+  G5_NONNULL(dv);
+  G5_NONNULL(ws);
+  uintptr_t align = 0;
+  for (const void* p : {dout, q, k, v, out, static_cast<const void*>(dq),
+                        static_cast<const void*>(dk), static_cast<const void*>(dv)})
+    align |= reinterpret_cast<uintptr_t>(p);
+  if (align % 16 != 0)
+    return fail(G5MOE_ERR_UNSUPPORTED, "every tensor of the backward must be 16-byte aligned");
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.o = static_cast<uint16_t*>(const_cast<void*>(out));
+  a.dout = static_cast<const uint16_t*>(dout);
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  a.do_tok = g.o_token_stride;
+  a.do_head = g.o_head_stride;
+  a.dq_tok = g.q_token_stride;
+  a.dq_head = g.q_head_stride;
+  a.dk_tok = g.k_token_stride;
+  a.dk_head = g.k_head_stride;
+  a.dv_tok = g.v_token_stride;
+  a.dv_head = g.v_head_stride;
+  a.lse = const_cast<float*>(softmax_lse);
+  const AttnBwdLayout w = attn_bwd_layout(options, s);
+  char* const base = static_cast<char*>(ws);
+  a.nl = reinterpret_cast<float*>(base + w.nl);
+  a.delta = reinterpret_cast<float*>(base + w.delta);
+  a.rowkey = reinterpret_cast<uint32_t*>(base + w.rowkey);
+  a.part = reinterpret_cast<float*>(base + w.part);
+  const bool wide = std::max({s.q_token_stride, s.k_token_stride, s.v_token_stride,
+                              g.o_token_stride}) >= (int64_t(1) << 24);
+  return hip_status(attn::launch_local_bwd(a, wide, dbias, reinterpret_cast<float*>(base + w.rel),
+                                           as_stream(stream)),
+                    "g5moe_attn_bwd");
+}
+
+static g5moe_status dropout_add(const void* x, const void* residual, void* out,
+                                const g5moe_dropout* dropout, float alpha, int64_t rows, int32_t d,
+                                int32_t dtype, void* stream, const char* where) {
+  DropoutParams drop;
+  G5_CHECK(dropout_params(dropout, &drop));
+  if (rows < 0 || d < 1)
+    return fail(G5MOE_ERR_INVALID_ARG, "rows %lld must be >= 0 and d %d >= 1", (long long)rows,
+                int(d));
+  if (dtype != G5MOE_DTYPE_BF16 && dtype != G5MOE_DTYPE_F32)
+    return fail(G5MOE_ERR_INVALID_ARG, "dtype %d is neither bf16 (0) nor f32 (1)", int(dtype));
+  // one 256-thread workgroup per 256 elements at most, in a grid of 32-bit size
+  if (rows > (int64_t(1) << 38) / d)
+    return fail(G5MOE_ERR_UNSUPPORTED, "%lld rows of %d elements exceed 2^38 elements",
+                (long long)rows, int(d));
+  if (rows == 0) return G5MOE_OK;
+  G5_NONNULL(x);
+  G5_NONNULL(out);
+  return hip_status(launch_dropout_add(x, residual, out, rows, d, dtype == G5MOE_DTYPE_F32, alpha,
+                                       drop, as_stream(stream)),
+                    where);
+}
+
+g5moe_status g5moe_dropout_add(const void* x, const void* residual, void* out,
+                               const g5moe_dropout* dropout, float alpha, int64_t rows, int32_t d,
+                               int32_t dtype, void* stream) {
+  if (rows > 0) G5_NONNULL(residual);
+  return dropout_add(x, residual, out, dropout, alpha, rows, d, dtype, stream,
+                     "g5moe_dropout_add");
+}
+
+g5moe_status g5moe_dropout_add_backward(const void* dout, void* dx, const g5moe_dropout* dropout,
+                                        float alpha, int64_t rows, int32_t d, int32_t dtype,
+                                        void* stream) {
+  return dropout_add(dout, nullptr, dx, dropout, alpha, rows, d, dtype, stream,
+                     "g5moe_dropout_add_backward");
 }
 
 }  // extern "C"

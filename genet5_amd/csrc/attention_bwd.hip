@@ -1,0 +1,660 @@
+// Backward of the attention: dQ, dK, dV and the gradient of the bucketed relative position
+// bias, for every form of the forward (full, window and sinks, ALiBi, bias table, dropout).
+//
+// With P_ij = exp(t_ij - lse_i) recomputed from the scores and the saved lse, m_ij the
+// dropout multiplier and delta_i = sum_d dO_id O_id (which equals sum_j P_ij m_ij dO_i.v_j):
+//   dV_j = sum_i m_ij P_ij dO_i
+//   dS_ij = P_ij (m_ij dO_i . v_j - delta_i)
+//   dQ_i = scale sum_j dS_ij k_j,   dK_j = scale sum_i dS_ij q_i
+//   dTable[b, h] = sum of dS_ij over the pairs with bucket(j - i) = b
+//
+// Two passes, so that every sum has a fixed order and no atomics: dq_kernel keeps 32 queries
+// per wave and walks the key tiles (3 products a tile: scores, dP, dQ), dkv_kernel keeps 32
+// keys per wave and walks the query tiles of each query head that shares the key head (4
+// products).  That is 7 products for the formulas' 5.  Both form the scores so that the
+// wave's own rows are the columns of the product (attn_tile.h): P and dS then are B operands
+// as they stand.  P and dS enter the products as bf16 (sums in fp32), as P does in the
+// forward.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_tile.h"
+
+namespace g5moe {
+namespace attn {
+namespace {
+
+constexpr int kBQ = 128;                       // own rows per workgroup, both kernels
+constexpr int kStageQ = 2 * kTileBytes;        // dq_kernel: K tile, V tile
+constexpr int kVecBytes = 1024;                // dkv_kernel: -lse, delta, row keys of a tile
+constexpr int kStageKV = 2 * kTileBytes + kVecBytes;
+
+// A wave's sums of dS by distance live in LDS, one table per half wave: the 32 lanes of a
+// half add to 32 different distances, and a wave's LDS operations keep their order, so the
+// sums do not depend on timing.
+constexpr int kGradTables = 8;
+
+template <int POS, bool DROP, bool DBIAS, bool WIDE>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+void dq_kernel(LocalArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  char* const ring = smem;
+  float* const tab = reinterpret_cast<float*>(smem + kStages * kStageQ);
+  const int n_tab = POS == kPosTable ? bias_entries(a.far) : 0;
+  float* const gtab = tab + n_tab;
+
+  const int z = blockIdx.z, hq = blockIdx.y;
+  if (z == a.n_seqs - 1)
+    zero_tail(a, a.dq, a.dq_tok, hq * a.dq_head, int(blockIdx.x), int(gridDim.x));
+  int s0, L;
+  sequence(a, z, s0, L);
+  const int q0 = blockIdx.x * kBQ;
+  if (q0 >= L) return;
+  const int hk = hq / a.group;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int wq = q0 + wave * kCols;
+  const int wq_hi = min(wq + kCols, L) - 1;
+  const int iq = wq + col;
+  const bool own = iq < L;
+  const int wl = min(a.wl, L), wr = min(a.wr, L), ns = min(a.ns, L);
+  const float sc = a.sc;
+  const float sl = POS == kPosAlibi ? a.slopes[hq] * kLog2e : 0.0f;
+
+  bf16x8 qf[4], dof[4];
+  float delta = 0.0f, nl = -kInf;  // a row past the end has probabilities of 0
+  {
+    const int64_t t = s0 + min(iq, L - 1);
+    load_own(qf, a.q + t * a.q_tok + hq * a.q_head, half, own, 0u);
+    load_own(dof, a.dout + t * a.do_tok + hq * a.do_head, half, own, 0u);
+    bf16x8 of[4];
+    load_own(of, a.o + t * a.o_tok + hq * a.o_head, half, own, 0u);
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        delta = __builtin_fmaf(float(dof[kc][e]), float(of[kc][e]), delta);
+    delta += __shfl_xor(delta, 32, 64);
+    const int64_t at = int64_t(hq) * a.total + t;
+    if (own) {
+      const float lse = a.lse[at];
+      // an empty row: every term is -inf, whatever is subtracted
+      nl = lse == -kInf ? 0.0f : -lse * kLog2e;
+    }
+    asm volatile("" : "+v"(nl));
+  }
+  uint32_t rkey = 0, thr = 0;
+  float up = 0.0f;
+  if constexpr (DROP) {
+    rkey = dropout_row_key(uint32_t(s0 + iq) * uint32_t(a.n_heads) + uint32_t(hq),
+                           a.drop.seed_lo, a.drop.seed_hi);
+    thr = min(a.drop.thr, 65535u) << 16;  // p = 1: the scale is 0
+    up = a.drop.scale;
+  }
+  if (own && half == 0) {
+    const int64_t at = int64_t(hq) * a.total + s0 + iq;
+    a.nl[at] = nl;
+    a.delta[at] = delta;
+    if constexpr (DROP) a.rowkey[at] = rkey;
+  }
+  if constexpr (POS == kPosTable) stage_bias(a, hq, tab);
+  if constexpr (DBIAS)
+    for (int x = tid; x < kGradTables * n_tab; x += 256) gtab[x] = 0.0f;
+  if constexpr (POS == kPosTable) __syncthreads();
+  const float far_l = POS == kPosTable ? tab[0] : 0.0f;
+  const float far_r = POS == kPosTable ? tab[n_tab - 1] : 0.0f;
+  BiasChunk bc;
+  if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
+
+  KeyTiles kt;
+  kt.init(q0, min(q0 + kBQ, L) - 1, L, wl, wr, ns);
+  TilePair<WIDE> tiles;
+  tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
+  FragReader fr;
+  fr.init(lane);
+  const char* const kbase =
+      reinterpret_cast<const char*>(a.k + int64_t(s0) * a.k_tok + hk * a.k_head);
+  const char* const vbase =
+      reinterpret_cast<const char*>(a.v + int64_t(s0) * a.v_tok + hk * a.v_head);
+  // past the last tile it goes out again, into a buffer that no later tile reads
+  int n_is = kt.first();
+  auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
+    tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff);
+    n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
+  };
+
+  f32x16 dq[2] = {f32x16{}, f32x16{}};
+  float sum_l = 0.0f, sum_r = 0.0f;  // dS at distances <= -far and >= far in plain tiles
+
+  // dS of 32 keys: half b of tile n, scores s and dP dp; c: the tile's constant bias.
+  auto grad = [&](auto mask_c, auto look_c, int n, int b, const f32x16& s, const f32x16& dp,
+                  float c, bool left, uint32_t (&pk)[8]) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_c)::value, LOOK = decltype(look_c)::value;
+    const int j0 = n * kRows + 32 * b + 4 * half;
+    const int lo = iq - wl - j0;
+    const uint32_t span = uint32_t(min(iq + wr, L - 1) - (iq - wl));
+    const int sink = ns - j0;
+    const float di = float(iq - j0);
+    const int rel0 = j0 - iq + a.far + kBiasPad;
+    const float* tb = tab + rel0;
+    float* gt = gtab + (2 * wave + half) * n_tab + rel0;
+    const uint32_t jp = uint32_t(j0) >> 1;
+    const float sub = nl + c;
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      uint32_t bits = 0;
+      if constexpr (DROP) bits = dropout_pair_bits(rkey, jp + uint32_t(8 * (r >> 2) + (r & 3)) / 2);
+      float ds[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int kr = 8 * (r >> 2) + (r & 3) + e;
+        const float x = s[r + e];
+        float t;
+        if constexpr (LOOK && POS == kPosTable)
+          t = __builtin_fmaf(x, sc, tb[kr]) + nl;
+        else if constexpr (LOOK && POS == kPosAlibi)
+          t = __builtin_fmaf(-sl, __builtin_fabsf(di - float(kr)), x * sc) + nl;
+        else
+          t = __builtin_fmaf(x, sc, sub);
+        if constexpr (MASK) t = (uint32_t(kr - lo) <= span || kr < sink) ? t : -kInf;
+        const float p = __builtin_amdgcn_exp2f(t);
+        float d = dp[r + e];
+        if constexpr (DROP) {
+          const float mult = (e == 0 ? bits << 16 : bits) >= thr ? up : 0.0f;
+          d = __builtin_fmaf(d, mult, -delta);
+        } else {
+          d -= delta;
+        }
+        ds[e] = p * d;
+        if constexpr (DBIAS) {
+          if constexpr (LOOK)
+            __hip_atomic_fetch_add(gt + kr, ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          else
+            sum += ds[e];
+        }
+      }
+      pk[r >> 1] = pack_bf16x2(ds[0], ds[1]);
+    }
+    if constexpr (DBIAS && !LOOK) {
+      sum_l += left ? sum : 0.0f;
+      sum_r += left ? 0.0f : sum;
+    }
+  };
+
+  int count = kt.s_end + kt.w_hi - kt.w_lo + 1;
+  int n = kt.first();
+  uint32_t boff = 0;
+#pragma unroll
+  for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageQ);
+  gemm::wait_vmcnt<(kStages - 1) * 4>();
+  __syncthreads();
+  for (; count > 0; --count, n = kt.next(n)) {
+    const int j0 = n * kRows, j1 = j0 + kRows - 1;
+    const bool some = wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
+    if (some) {
+      const f32x16 zero16 = {};
+      const char* const K = ring + boff;
+      const char* const V = K + kTileBytes;
+      const bool all = j1 < L && ((j0 >= wq_hi - wl && j1 <= wq + wr) || j1 < ns);
+      using T_ = std::true_type;
+      using F_ = std::false_type;
+      float c = 0.0f;
+      bool look = false, left = false, before = false;
+      if constexpr (POS == kPosTable) {
+        left = j1 - wq <= -a.far;
+        look = !left && j0 - wq_hi < a.far;
+        c = left ? far_l : far_r;
+      }
+      if constexpr (POS == kPosAlibi) {
+        before = j1 <= wq;
+        look = !(bc.ok && (before || j0 >= wq_hi));
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int kc = 0; kc < 4; ++kc)
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(K, b, kc), qf[kc],
+                                                      kc == 0 ? zero16 : s, 0, 0, 0);
+#pragma unroll
+        for (int kc = 0; kc < 4; ++kc)
+          dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(V, b, kc), dof[kc],
+                                                       kc == 0 ? zero16 : dp, 0, 0, 0);
+        uint32_t pk[8];
+        if constexpr (POS == kPosAlibi)
+          if (!look) s = bc.add_half(s, b, float(iq - j0), before);
+        if (POS != kPosNone && look) {
+          if (all)
+            grad(F_{}, T_{}, n, b, s, dp, 0.0f, false, pk);
+          else
+            grad(T_{}, T_{}, n, b, s, dp, 0.0f, false, pk);
+        } else {
+          if (all)
+            grad(F_{}, F_{}, n, b, s, dp, c, left, pk);
+          else
+            grad(T_{}, F_{}, n, b, s, dp, c, left, pk);
+        }
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const bf16x8 df = chunk(pk, cc);
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb)
+            dq[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.trans(K, 2 * b + cc, mb), df,
+                                                             dq[mb], 0, 0, 0);
+        }
+      }
+    }
+    // the next stage landed, and every wave has read all of this one
+    gemm::wait_vmcnt<(kStages - 2) * 4>();
+    __syncthreads();
+    issue(boff);
+    boff = boff + kStageQ == kStages * kStageQ ? 0 : boff + kStageQ;
+  }
+  // refills past the last tile may still be landing in this workgroup's LDS
+  gemm::wait_vmcnt<0>();
+
+  if (own) {
+    uint16_t* op = a.dq + int64_t(s0 + iq) * a.dq_tok + hq * a.dq_head + 4 * half;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint2 w;
+        w.x = pack_bf16x2(dq[mb][4 * q] * a.scale, dq[mb][4 * q + 1] * a.scale);
+        w.y = pack_bf16x2(dq[mb][4 * q + 2] * a.scale, dq[mb][4 * q + 3] * a.scale);
+        *reinterpret_cast<uint2*>(op + 32 * mb + 8 * q) = w;
+      }
+  }
+
+  if constexpr (DBIAS) {
+    // the workgroup's sums by distance, clamped to +-far, in a fixed order: the tables in
+    // order, then what lies past far, then the plain tiles' sums
+    __shared__ float ends[2][4];
+    sum_l = butterfly_sum64(sum_l);
+    sum_r = butterfly_sum64(sum_r);
+    if (lane == 0) {
+      ends[0][wave] = sum_l;
+      ends[1][wave] = sum_r;
+    }
+    __syncthreads();
+    auto column = [&](int x) {
+      float v = 0.0f;
+#pragma unroll
+      for (int t = 0; t < kGradTables; ++t) v += gtab[t * n_tab + x];
+      return v;
+    };
+    const int E = 2 * a.far + 1;
+    float* out = a.part + (int64_t(hq) * gridDim.z * gridDim.x + int64_t(z) * gridDim.x +
+                           blockIdx.x) * E;
+    for (int x = tid; x < E; x += 256)
+      if (x != 0 && x != E - 1) out[x] = column(kBiasPad + x);
+    if (wave < 2) {
+      // entries 0 .. kBiasPad (left) or the last kBiasPad + 1 (right)
+      const int from = wave == 0 ? 0 : kBiasPad + E - 1;
+      float v = column(from + lane);
+      if (lane < kBiasPad + 1 - 64) v += column(from + 64 + lane);
+      v = butterfly_sum64(v);
+      v += ends[wave][0] + ends[wave][1] + (ends[wave][2] + ends[wave][3]);
+      if (lane == 0) out[wave == 0 ? 0 : E - 1] = v;
+    }
+  }
+}
+
+// 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).
+template <int POS, bool DROP, bool WIDE>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+void dkv_kernel(LocalArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  char* const ring = smem;
+  float* const tab = reinterpret_cast<float*>(smem + kStages * kStageKV);
+
+  const int z = blockIdx.z, hk = blockIdx.y;
+  if (z == a.n_seqs - 1) {
+    zero_tail(a, a.dk, a.dk_tok, hk * a.dk_head, int(blockIdx.x), int(gridDim.x));
+    zero_tail(a, a.dv, a.dv_tok, hk * a.dv_head, int(blockIdx.x), int(gridDim.x));
+  }
+  int s0, L;
+  sequence(a, z, s0, L);
+  const int k0 = blockIdx.x * kBQ;
+  if (k0 >= L) return;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int wk = k0 + wave * kCols;               // the wave's keys: wk .. wk_hi
+  const int wk_hi = min(wk + kCols, L) - 1;
+  const int jk = wk + col;
+  const bool own = jk < L;
+  const int wl = min(a.wl, L), wr = min(a.wr, L), ns = min(a.ns, L);
+  const float sc = a.sc;
+
+  bf16x8 kf[4], vf[4];
+  load_own(kf, a.k + int64_t(s0 + min(jk, L - 1)) * a.k_tok + hk * a.k_head, half, own, 0u);
+  load_own(vf, a.v + int64_t(s0 + min(jk, L - 1)) * a.v_tok + hk * a.v_head, half, own, 0u);
+  uint32_t thr = 0, golden_c = 0;
+  float up = 0.0f;
+  if constexpr (DROP) {
+    thr = min(a.drop.thr, 65535u) << 16;
+    golden_c = (uint32_t(jk) >> 1) * 0x9e3779b9u;
+    up = a.drop.scale;
+  }
+
+  // query tiles that see one of the workgroup's keys
+  const int k_hi = min(k0 + kBQ, L) - 1;
+  const int t_lo = k0 < ns ? 0 : max(k0 - wr, 0) / kRows;
+  const int t_hi = k0 < ns ? (L - 1) / kRows : min(k_hi + wl, L - 1) / kRows;
+
+  TilePair<WIDE> tiles;
+  tiles.init(ring, wave, lane, L, a.q_tok * 2, a.do_tok * 2);
+  FragReader fr;
+  fr.init(lane);
+  const uint32_t vec_off[2] = {uint32_t(lane) * 4, uint32_t(min(lane, tiles.lastrow)) * 4};
+  const uint32_t vec_lds = gemm::lds_addr(ring) + 2 * kTileBytes + uint32_t(wave) * 256;
+  const float* const vsrc = wave == 1 ? a.delta
+                            : (DROP && wave == 2) ? reinterpret_cast<const float*>(a.rowkey)
+                                                  : a.nl;
+  // tiles of (head, number) in order; past the last one it goes out again
+  int h_is = hk * a.group, n_is = t_lo;
+  const int h_end = h_is + a.group;
+  auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
+    const int h = __builtin_amdgcn_readfirstlane(h_is), n = __builtin_amdgcn_readfirstlane(n_is);
+    tiles.issue(reinterpret_cast<const char*>(a.q + int64_t(s0) * a.q_tok + h * a.q_head),
+                reinterpret_cast<const char*>(a.dout + int64_t(s0) * a.do_tok + h * a.do_head),
+                n, boff);
+    gemm::lds_dma4_s(vsrc + int64_t(h) * a.total + s0 + int64_t(n) * kRows,
+                     n == tiles.last ? vec_off[1] : vec_off[0], vec_lds + boff);
+    const bool wrap = n_is == t_hi, more = h_is + 1 < h_end;
+    n_is = wrap ? (more ? t_lo : n_is) : n_is + 1;
+    h_is = wrap && more ? h_is + 1 : h_is;
+  };
+
+  f32x16 dk[2] = {f32x16{}, f32x16{}}, dv[2] = {f32x16{}, f32x16{}};
+  float sl = 0.0f, far_l = 0.0f, far_r = 0.0f;
+  BiasChunk bc;
+
+  // P (dropped) and dS of 32 queries: half b of tile n, scores s and dP dp.
+  auto grad = [&](auto mask_c, auto look_c, int n, int b, const f32x16& s, const f32x16& dp,
+                  float c, uint32_t boff, uint32_t (&pkp)[8], uint32_t (&pkd)[8])
+      __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_c)::value, LOOK = decltype(look_c)::value;
+    const int i0 = n * kRows + 32 * b + 4 * half;
+    // tile offsets of the queries that see key jk: lo .. lo + span
+    const bool sink = jk < ns;
+    const int q_lo = sink ? 0 : max(jk - wr, 0);
+    const int q_hi = sink ? L - 1 : min(jk + wl, L - 1);
+    const int lo = q_lo - i0;
+    const uint32_t span = uint32_t(q_hi - q_lo);
+    const float dj = float(jk - i0);
+    const float* tb = tab + (jk - i0 - 31 + a.far + kBiasPad);
+    const float* vec =
+        reinterpret_cast<const float*>(ring + boff + 2 * kTileBytes) + 32 * b + 4 * half;
+    uint32_t hb[8];
+    if constexpr (DROP) {
+      // a pair of lanes being the two columns of one hash, even lanes hash for the first 16
+      // queries, odd lanes for the others
+      const uint32_t* keys = reinterpret_cast<const uint32_t*>(vec) + 128 + 16 * (lane & 1);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const u32x4 kk = *reinterpret_cast<const u32x4*>(keys + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hb[4 * q + e] = fmix32(kk[e] + golden_c);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 nl4 = *reinterpret_cast<const f32x4*>(vec + 8 * q);
+      const f32x4 dl4 = *reinterpret_cast<const f32x4*>(vec + 64 + 8 * q);
+      float pd[4], ds[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * q + e;
+        const int qr = 8 * q + e;
+        const float x = s[r];
+        float t;
+        if constexpr (LOOK && POS == kPosTable)
+          t = __builtin_fmaf(x, sc, nl4[e]) + tb[31 - qr];
+        else if constexpr (LOOK && POS == kPosAlibi)
+          t = __builtin_fmaf(-sl, __builtin_fabsf(dj - float(qr)),
+                             __builtin_fmaf(x, sc, nl4[e]));
+        else if constexpr (POS == kPosTable)
+          t = __builtin_fmaf(x, sc, nl4[e]) + c;
+        else
+          t = __builtin_fmaf(x, sc, nl4[e]);
+        if constexpr (MASK) t = uint32_t(qr - lo) <= span ? t : -kInf;
+        const float p = __builtin_amdgcn_exp2f(t);
+        float d = dp[r];
+        if constexpr (DROP) {
+          const uint32_t other =
+              __builtin_amdgcn_update_dpp(0u, hb[r & 7], 0xb1, 0xf, 0xf, false);  // lane ^ 1
+          const uint32_t bits = (lane & 1) == (q >> 1) ? hb[r & 7] : other;
+          const float mult = ((lane & 1) ? bits : bits << 16) >= thr ? up : 0.0f;
+          pd[e] = p * mult;
+          d = __builtin_fmaf(d, mult, -dl4[e]);
+        } else {
+          pd[e] = p;
+          d -= dl4[e];
+        }
+        ds[e] = p * d;
+      }
+      pkp[2 * q] = pack_bf16x2(pd[0], pd[1]);
+      pkp[2 * q + 1] = pack_bf16x2(pd[2], pd[3]);
+      pkd[2 * q] = pack_bf16x2(ds[0], ds[1]);
+      pkd[2 * q + 1] = pack_bf16x2(ds[2], ds[3]);
+    }
+  };
+
+  uint32_t boff = 0;
+#pragma unroll
+  for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageKV);
+  gemm::wait_vmcnt<(kStages - 1) * 5>();
+  __syncthreads();
+  for (int h = hk * a.group; h < h_end; ++h) {
+    if constexpr (POS == kPosTable) {
+      __syncthreads();  // the previous head's table is read no more
+      stage_bias(a, h, tab);
+      __syncthreads();
+      far_l = tab[0];
+      far_r = tab[bias_entries(a.far) - 1];
+    }
+    if constexpr (POS == kPosAlibi) {
+      sl = a.slopes[h] * kLog2e;
+      bc.init(sl, sc, lane);
+    }
+    for (int n = t_lo; n <= t_hi; ++n) {
+      const int i0 = n * kRows, i1 = i0 + kRows - 1;
+      const bool some =
+          wk < L && ((i0 <= wk_hi + wl && i1 >= wk - wr) || wk < ns);
+      if (some) {
+        const f32x16 zero16 = {};
+        const char* const Q = ring + boff;
+        const char* const D = Q + kTileBytes;
+        const bool all = i1 < L && ((i1 <= wk + wl && i0 >= wk_hi - wr) || wk_hi < ns);
+        using T_ = std::true_type;
+        using F_ = std::false_type;
+        float c = 0.0f;
+        bool look = false, before = false;
+        if constexpr (POS == kPosTable) {
+          const bool left = wk + kCols - 1 - i0 <= -a.far, right = wk - i1 >= a.far;
+          look = !left && !right;
+          c = left ? far_l : far_r;
+        }
+        if constexpr (POS == kPosAlibi) {
+          before = i1 <= wk;
+          look = !(bc.ok && (before || i0 >= wk + kCols - 1));
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          f32x16 s, dp;
+#pragma unroll
+          for (int kc = 0; kc < 4; ++kc)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(Q, b, kc), kf[kc],
+                                                        kc == 0 ? zero16 : s, 0, 0, 0);
+#pragma unroll
+          for (int kc = 0; kc < 4; ++kc)
+            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(D, b, kc), vf[kc],
+                                                         kc == 0 ? zero16 : dp, 0, 0, 0);
+          uint32_t pkp[8], pkd[8];
+          if constexpr (POS == kPosAlibi)
+            if (!look) s = bc.add_half(s, b, float(jk - i0), before);
+          if (POS != kPosNone && look) {
+            if (all)
+              grad(F_{}, T_{}, n, b, s, dp, 0.0f, boff, pkp, pkd);
+            else
+              grad(T_{}, T_{}, n, b, s, dp, 0.0f, boff, pkp, pkd);
+          } else {
+            if (all)
+              grad(F_{}, F_{}, n, b, s, dp, c, boff, pkp, pkd);
+            else
+              grad(T_{}, F_{}, n, b, s, dp, c, boff, pkp, pkd);
+          }
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const bf16x8 pf = chunk(pkp, cc), df = chunk(pkd, cc);
+#pragma unroll
+            for (int mb = 0; mb < 2; ++mb) {
+              dv[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.trans(D, 2 * b + cc, mb), pf,
+                                                               dv[mb], 0, 0, 0);
+              dk[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.trans(Q, 2 * b + cc, mb), df,
+                                                               dk[mb], 0, 0, 0);
+            }
+          }
+        }
+      }
+      // the next stage landed, and every wave has read all of this one
+      gemm::wait_vmcnt<(kStages - 2) * 5>();
+      __syncthreads();
+      issue(boff);
+      boff = boff + kStageKV == kStages * kStageKV ? 0 : boff + kStageKV;
+    }
+  }
+  // refills past the last tile may still be landing in this workgroup's LDS
+  gemm::wait_vmcnt<0>();
+
+  if (own) {
+    const int64_t t = s0 + jk;
+    uint16_t* kp = a.dk + t * a.dk_tok + hk * a.dk_head + 4 * half;
+    uint16_t* vp = a.dv + t * a.dv_tok + hk * a.dv_head + 4 * half;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint2 w;
+        w.x = pack_bf16x2(dk[mb][4 * q] * a.scale, dk[mb][4 * q + 1] * a.scale);
+        w.y = pack_bf16x2(dk[mb][4 * q + 2] * a.scale, dk[mb][4 * q + 3] * a.scale);
+        *reinterpret_cast<uint2*>(kp + 32 * mb + 8 * q) = w;
+        w.x = pack_bf16x2(dv[mb][4 * q], dv[mb][4 * q + 1]);
+        w.y = pack_bf16x2(dv[mb][4 * q + 2], dv[mb][4 * q + 3]);
+        *reinterpret_cast<uint2*>(vp + 32 * mb + 8 * q) = w;
+      }
+  }
+}
+
+// The workgroups' sums by distance added up in order: rel[h, x].  Four waves take every
+// fourth workgroup each.
+__global__ __launch_bounds__(256) void bias_sum_kernel(LocalArgs a, int nx, int E, float* rel) {
+  __shared__ float red[4][64];
+  const int h = blockIdx.y;
+  const int x = blockIdx.x * 64 + (threadIdx.x & 63);
+  const int wave = threadIdx.x >> 6;
+  float v = 0.0f;
+  if (x < E)
+    for (int z = 0; z < a.n_seqs; ++z) {
+      int s0, L;
+      sequence(a, z, s0, L);
+      const int nq = min((L + kBQ - 1) / kBQ, nx);
+      const float* p = a.part + ((int64_t(h) * a.n_seqs + z) * nx) * E + x;
+      for (int q = wave; q < nq; q += 4) v += p[int64_t(q) * E];
+    }
+  red[wave][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (wave == 0 && x < E)
+    rel[int64_t(h) * E + x] = (red[0][threadIdx.x] + red[1][threadIdx.x]) +
+                              (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// dTable[b, h]: the sums of the distances in bucket b, in order.
+__global__ __launch_bounds__(256) void bias_bucket_kernel(LocalArgs a, int E, const float* rel,
+                                                          void* dbias) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* const v = reinterpret_cast<float*>(smem);
+  int* const bk = reinterpret_cast<int*>(v + E);
+  const int h = blockIdx.x;
+  for (int x = threadIdx.x; x < E; x += 256) {
+    v[x] = rel[int64_t(h) * E + x];
+    bk[x] = min(max(a.bucket_of[x], 0), a.n_buckets - 1);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.n_buckets; b += 256) {
+    float sum = 0.0f;
+    for (int x = 0; x < E; ++x) sum += bk[x] == b ? v[x] : 0.0f;
+    const int64_t at = int64_t(b) * a.n_heads + h;
+    if (a.bias_bf16)
+      static_cast<uint16_t*>(dbias)[at] = f32_to_bf16_bits(sum);
+    else
+      static_cast<float*>(dbias)[at] = sum;
+  }
+}
+
+}  // namespace
+
+int64_t bwd_part_floats(int max_seqlen, int n_seqs, int n_heads, int far) {
+  return int64_t((max_seqlen + kBQ - 1) / kBQ) * n_seqs * n_heads * (2 * far + 1);
+}
+
+hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* rel,
+                            hipStream_t st) {
+  const unsigned nx = unsigned((a.max_len + kBQ - 1) / kBQ);
+  const bool table = a.bias != nullptr, grad = dbias != nullptr;
+  const size_t tab = table ? size_t(bias_entries(a.far)) * 4 : 0;
+  const size_t lds_q = size_t(kStages) * kStageQ + tab * (grad ? 1 + kGradTables : 1);
+  const size_t lds_kv = size_t(kStages) * kStageKV + tab;
+  auto launch = [&](auto kernel, int heads, size_t lds) {
+    // a large max distance needs more than the default limit of 64 KB
+    if (lds > 65536 - 2048) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               int(lds));
+      if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kernel, dim3(nx, unsigned(heads), unsigned(a.n_seqs)), dim3(256), lds, st,
+                       a);
+    return hipGetLastError();
+  };
+  const int hkv = a.n_heads / a.group;
+  auto run = [&](auto pos, auto drop, auto w) {
+    constexpr int P = decltype(pos)::value;
+    constexpr bool D = decltype(drop)::value, W = decltype(w)::value;
+    hipError_t e;
+    if constexpr (P == kPosTable)
+      e = grad ? launch(dq_kernel<P, D, true, W>, a.n_heads, lds_q)
+               : launch(dq_kernel<P, D, false, W>, a.n_heads, lds_q);
+    else
+      e = launch(dq_kernel<P, D, false, W>, a.n_heads, lds_q);
+    if (e != hipSuccess) return e;
+    return launch(dkv_kernel<P, D, W>, hkv, lds_kv);
+  };
+  using T_ = std::true_type;
+  using F_ = std::false_type;
+  auto pick = [&](auto pos) {
+    if (a.drop.on) return wide ? run(pos, T_{}, T_{}) : run(pos, T_{}, F_{});
+    return wide ? run(pos, F_{}, T_{}) : run(pos, F_{}, F_{});
+  };
+  hipError_t e = table ? pick(std::integral_constant<int, kPosTable>{})
+                 : a.slopes != nullptr ? pick(std::integral_constant<int, kPosAlibi>{})
+                                       : pick(std::integral_constant<int, kPosNone>{});
+  if (e != hipSuccess || !grad) return e;
+  const int E = 2 * a.far + 1;
+  hipLaunchKernelGGL(bias_sum_kernel, dim3(unsigned((E + 63) / 64), unsigned(a.n_heads)),
+                     dim3(256), 0, st, a, int(nx), E, rel);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(bias_bucket_kernel, dim3(unsigned(a.n_heads)), dim3(256), size_t(E) * 8, st,
+                     a, E, rel, dbias);
+  return hipGetLastError();
+}
+
+}  // namespace attn
+}  // namespace g5moe

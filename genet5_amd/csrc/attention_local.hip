@@ -1,0 +1,314 @@
+// Attention with a sliding window, sink tokens, a bucketed relative position bias (or
+// ALiBi) and dropout on the probabilities: the forward pass.
+//
+// For query i of a sequence of length L (positions inside the sequence)
+//   visible keys  V(i) = { j < L : i - wl <= j <= i + wr  or  j < ns }
+//   t_ij = scale q_i . k_j + bias_ij,  P = softmax of t over V(i)
+//   O_i  = sum_j m_ij P_ij v_j,        lse_i = log sum_j exp t_ij
+// with m_ij the dropout multiplier (1 without dropout), so the softmax is normalised by
+// the undropped sum.  A row whose every visible term is -inf (a bias of -inf) gives O = 0
+// and lse = -inf.
+//
+// Work split: one workgroup of four waves per (128 queries, head, sequence), a wave holding
+// 32 queries; the 64-key tiles that any of the 128 queries sees (the sinks' tiles, then the
+// window's) stream through a ring of three in LDS, filled by LDS DMA.  One pass over the
+// keys with the running maximum and sum of the softmax, scores transposed (S^T = K Q^T) so
+// that a query's statistics live in two lanes and the probabilities are the B operand of
+// O^T += V^T P^T as they stand (attn_tile.h).  Per wave a tile is skipped (nothing of it is
+// visible to the wave's queries), plain (all of it visible, the bias constant or linear), or
+// takes the per-element path (MASK: an edge of the window, the sinks or the sequence; LOOK:
+// the bias from the table, or ALiBi across the diagonal).
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_tile.h"
+
+namespace g5moe {
+namespace attn {
+namespace {
+
+constexpr int kBQ = 128;
+constexpr int kStageBytes = 2 * kTileBytes;
+
+template <int POS, bool DROP, bool WIDE>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+void local_fwd_kernel(LocalArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  char* const ring = smem;
+  float* const tab = reinterpret_cast<float*>(smem + kStages * kStageBytes);
+
+  const int z = blockIdx.z, hq = blockIdx.y;
+  if (z == a.n_seqs - 1)
+    zero_tail(a, a.o, a.o_tok, hq * a.o_head, int(blockIdx.x), int(gridDim.x));
+  int s0, L;
+  sequence(a, z, s0, L);
+  const int q0 = blockIdx.x * kBQ;
+  if (q0 >= L) return;
+  const int hk = hq / a.group;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int wq = q0 + wave * kCols;               // the wave's queries: wq .. wq_hi
+  const int wq_hi = min(wq + kCols, L) - 1;
+  const int iq = wq + col;
+  const int wl = min(a.wl, L), wr = min(a.wr, L), ns = min(a.ns, L);
+  // a negative scale is taken as its magnitude on negated queries (the same products)
+  const float sc = __builtin_fabsf(a.sc);
+  const float sl = POS == kPosAlibi ? a.slopes[hq] * kLog2e : 0.0f;
+
+  bf16x8 qf[4];
+  load_own(qf, a.q + int64_t(s0 + min(iq, L - 1)) * a.q_tok + hq * a.q_head, half, iq < L,
+           a.sc < 0.0f ? 0x80008000u : 0u);
+  if constexpr (POS == kPosTable) {
+    stage_bias(a, hq, tab);
+    __syncthreads();
+  }
+  const float far_l = POS == kPosTable ? tab[0] : 0.0f;
+  const float far_r = POS == kPosTable ? tab[bias_entries(a.far) - 1] : 0.0f;
+  BiasChunk bc;
+  if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
+
+  uint32_t rkey = 0, thr = 0;
+  if constexpr (DROP) {
+    rkey = dropout_row_key(uint32_t(s0 + iq) * uint32_t(a.n_heads) + uint32_t(hq),
+                           a.drop.seed_lo, a.drop.seed_hi);
+    thr = min(a.drop.thr, 65535u) << 16;  // p = 1: the scale is 0
+  }
+
+  KeyTiles kt;
+  kt.init(q0, min(q0 + kBQ, L) - 1, L, wl, wr, ns);
+  TilePair<WIDE> tiles;
+  tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
+  FragReader fr;
+  fr.init(lane);
+  const char* const kbase =
+      reinterpret_cast<const char*>(a.k + int64_t(s0) * a.k_tok + hk * a.k_head);
+  const char* const vbase =
+      reinterpret_cast<const char*>(a.v + int64_t(s0) * a.v_tok + hk * a.v_head);
+
+  // The next tile to load; past the last one it goes out again, into a buffer that no later
+  // tile reads, so that every step issues the same number of loads.
+  int n_is = kt.first();
+  auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
+    tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff);
+    n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
+  };
+  bf16x8 kf[2][4];
+  auto load_kf = [&](uint32_t boff) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) kf[b][kc] = fr.row(ring + boff, b, kc);
+  };
+
+  f32x16 o[2] = {f32x16{}, f32x16{}};
+  float m = -kInf, psum = 0.0f;
+  float ms = 0.0f;  // what the exponents subtract: m, or 0 while every term was -inf
+  f32x16 s[2];
+  uint32_t pk[2][8];
+
+  auto advance = [&](float mx) __attribute__((always_inline)) {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
+                                                     false, false);
+    mx = __builtin_fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    const float m_new = __builtin_fmaxf(m, mx);
+    if (__ballot(m_new != m) != 0) {
+      ms = m_new == -kInf ? 0.0f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m - ms);
+      m = m_new;
+      psum *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[mb][r] *= alpha;
+    }
+  };
+  // The probabilities of the scores in s, tile n.  c: the tile's constant bias (neither MASK
+  // nor LOOK: added here; else part of the terms already).
+  auto softmax = [&](auto plain_c, int n, float c) __attribute__((always_inline)) {
+    constexpr bool PLAIN = decltype(plain_c)::value;
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2)
+        mx = __builtin_fmaxf(__builtin_fmaxf(mx, s[b][r]), s[b][r + 1]);
+    if constexpr (PLAIN)
+      advance(POS == kPosTable ? __builtin_fmaf(mx, sc, c) : mx * sc);
+    else
+      advance(mx);
+    const float sub = POS == kPosTable && PLAIN ? c - ms : -ms;
+    const uint32_t jp = uint32_t(n * kRows + 4 * half) >> 1;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        float p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float t = PLAIN ? __builtin_fmaf(s[b][r + e], sc, sub) : s[b][r + e] + sub;
+          p[e] = __builtin_amdgcn_exp2f(t);
+          sum += p[e];
+        }
+        if constexpr (DROP) {
+          const uint32_t bits =
+              dropout_pair_bits(rkey, jp + uint32_t(32 * b + 8 * (r >> 2) + (r & 3)) / 2);
+          p[0] = (bits << 16) >= thr ? p[0] : 0.0f;
+          p[1] = bits >= thr ? p[1] : 0.0f;
+        }
+        pk[b][r >> 1] = pack_bf16x2(p[0], p[1]);
+      }
+    psum += sum;
+  };
+  // Per-element terms in place of the scores.
+  auto terms = [&](auto mask_c, auto look_c, int n, float c) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_c)::value, LOOK = decltype(look_c)::value;
+    const int j0 = n * kRows + 4 * half;   // the lane's first key
+    const int lo = iq - wl - j0;           // window: tile offsets lo .. lo + span
+    const uint32_t span = uint32_t(min(iq + wr, L - 1) - (iq - wl));
+    const int sink = ns - j0;
+    const float di = float(iq - j0);
+    const float* tb = tab + (j0 - iq + a.far + kBiasPad);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int kr = 32 * b + 8 * (r >> 2) + (r & 3);
+        float t;
+        if constexpr (LOOK && POS == kPosTable)
+          t = __builtin_fmaf(s[b][r], sc, tb[kr]);
+        else if constexpr (LOOK && POS == kPosAlibi)
+          t = __builtin_fmaf(-sl, __builtin_fabsf(di - float(kr)), s[b][r] * sc);
+        else
+          t = __builtin_fmaf(s[b][r], sc, c);
+        if constexpr (MASK) t = (uint32_t(kr - lo) <= span || kr < sink) ? t : -kInf;
+        s[b][r] = t;
+      }
+  };
+
+  int count = kt.s_end + kt.w_hi - kt.w_lo + 1;
+  int n = kt.first();
+  uint32_t boff = 0;
+#pragma unroll
+  for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageBytes);
+  gemm::wait_vmcnt<(kStages - 1) * 4>();
+  __syncthreads();
+  load_kf(0);
+  for (; count > 0; --count, n = kt.next(n)) {
+    const int j0 = n * kRows, j1 = j0 + kRows - 1;
+    // what the wave's queries see of the tile
+    const bool some = wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
+    bf16x8 vf[4][2];
+    if (some) {
+      const f32x16 zero16 = {};
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][kc], qf[kc],
+                                                         kc == 0 ? zero16 : s[b], 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) vf[c][mb] = fr.trans(ring + boff + kTileBytes, c, mb);
+      const bool all = j1 < L && ((j0 >= wq_hi - wl && j1 <= wq + wr) || j1 < ns);
+      using T_ = std::true_type;
+      using F_ = std::false_type;
+      float c = 0.0f;
+      bool look = false;
+      if constexpr (POS == kPosTable) {
+        const bool left = j1 - wq <= -a.far, right = j0 - wq_hi >= a.far;
+        look = !left && !right;
+        c = left ? far_l : far_r;
+      }
+      if constexpr (POS == kPosAlibi) {
+        const bool before = j1 <= wq, after = j0 >= wq_hi;
+        look = !(bc.ok && (before || after));
+        if (!look) bc.add(s, float(iq - j0), before);
+      }
+      if (all && !look) {
+        softmax(T_{}, n, c);
+      } else {
+        if (POS == kPosNone || !look)
+          terms(T_{}, F_{}, n, c);
+        else if (all)
+          terms(F_{}, T_{}, n, c);
+        else
+          terms(T_{}, T_{}, n, c);
+        softmax(F_{}, n, c);
+      }
+    }
+    // the next stage landed, and every wave has read all of this one
+    gemm::wait_vmcnt<(kStages - 2) * 4>();
+    __syncthreads();
+    issue(boff);
+    boff = boff + kStageBytes == kStages * kStageBytes ? 0 : boff + kStageBytes;
+    load_kf(boff);
+    if (some) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bf16x8 pf = chunk(pk[c >> 1], c & 1);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+          o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[c][mb], pf, o[mb], 0, 0, 0);
+      }
+    }
+  }
+  // refills past the last tile may still be landing in this workgroup's LDS
+  gemm::wait_vmcnt<0>();
+
+  if (iq < L) {
+    const float l = psum + __shfl_xor(psum, 32, 64);
+    const float inv = l == 0.0f ? 0.0f : (DROP ? a.drop.scale : 1.0f) / l;
+    uint16_t* op = a.o + int64_t(s0 + iq) * a.o_tok + hq * a.o_head + 4 * half;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint2 w;
+        w.x = pack_bf16x2(o[mb][4 * q] * inv, o[mb][4 * q + 1] * inv);
+        w.y = pack_bf16x2(o[mb][4 * q + 2] * inv, o[mb][4 * q + 3] * inv);
+        *reinterpret_cast<uint2*>(op + 32 * mb + 8 * q) = w;
+      }
+    if (a.lse != nullptr && half == 0)
+      a.lse[int64_t(hq) * a.total + s0 + iq] = l == 0.0f ? -kInf : (m + __builtin_log2f(l)) * kLn2;
+  }
+}
+
+__global__ __launch_bounds__(256) void zero_behind_kernel(LocalArgs a) {
+  zero_tail(a, a.o, a.o_tok, int64_t(blockIdx.y) * a.o_head, int(blockIdx.x), int(gridDim.x));
+}
+
+}  // namespace
+
+hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL(zero_behind_kernel, dim3(16, unsigned(a.n_heads)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st) {
+  const dim3 grid(unsigned((a.max_len + kBQ - 1) / kBQ), unsigned(a.n_heads),
+                  unsigned(a.n_seqs));
+  const size_t lds =
+      size_t(kStages) * kStageBytes + (a.bias != nullptr ? bias_entries(a.far) * 4 : 0);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a); };
+  auto pick = [&](auto pos) {
+    constexpr int P = decltype(pos)::value;
+    if (a.drop.on)
+      wide ? launch(local_fwd_kernel<P, true, true>) : launch(local_fwd_kernel<P, true, false>);
+    else
+      wide ? launch(local_fwd_kernel<P, false, true>) : launch(local_fwd_kernel<P, false, false>);
+  };
+  if (a.bias != nullptr)
+    pick(std::integral_constant<int, kPosTable>{});
+  else if (a.slopes != nullptr)
+    pick(std::integral_constant<int, kPosAlibi>{});
+  else
+    pick(std::integral_constant<int, kPosNone>{});
+  return hipGetLastError();
+}
+
+}  // namespace attn
+}  // namespace g5moe

@@ -283,6 +283,10 @@ __device__ __forceinline__ int pad_start_lane(int ol, int n_experts, int kmax) {
   return lane == 0 ? 0 : ex;
 }
 
+// residual = nullptr: the backward, out = alpha m x.
+hipError_t launch_dropout_add(const void* x, const void* residual, void* out, int64_t rows, int d,
+                              bool f32, float alpha, const DropoutParams& drop, hipStream_t st);
+
 // ---- device helpers -------------------------------------------------------
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t b) {
   return __uint_as_float(b << 16);

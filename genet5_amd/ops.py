@@ -41,6 +41,16 @@ def _stream(device: torch.device):
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """_lib.call with `device` current: a launch belongs to the current device, whichever
+    device its stream and tensors are on."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args)
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args)
+
+
 def _dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return _lib.DTYPE_BF16

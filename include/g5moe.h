@@ -90,7 +90,8 @@ const char* g5moe_last_error(void);
  * signature changed.  2.2: g5moe_route (router and dispatch in two launches,
  * used by g5moe_forward); the workspace gains its per-chunk count region.
  * 2.3: g5moe_add_rmsnorm_route (the same for the residual add + RMSNorm +
- * router). */
+ * router).  2.4: g5moe_attn_local_fwd, g5moe_attn_bwd, g5moe_dropout_add and
+ * g5moe_dropout_add_backward. */
 int32_t g5moe_version(void);
 
 /* Bytes of workspace the stage entry points and g5moe_forward need for `shape`.
@@ -616,6 +617,85 @@ g5moe_status g5moe_attn_varlen_fwd(const void* q, const void* k, const void* v, 
                                    const int32_t* cu_seqlens, const float* alibi_slopes,
                                    float softmax_scale, float* softmax_lse, void* ws,
                                    const g5moe_attn_shape* shape, void* stream);
+
+/* ---- Attention with a window, sinks, a learned position bias, dropout; backward ----
+ * What flash_attn_varlen_func(..., dropout_p, window_size=...) computes on the training
+ * path of FlashAttention.forward (lib/blocks/_flash_att.py:76-96), with tokens at the start
+ * of each sequence that stay visible and a bias table over bucketed relative positions.
+ *
+ * For query i and key j of one sequence (positions from its start):
+ *   visible  i - window_left <= j <= i + window_right  or  j < sink_tokens
+ *   t[i, j] = softmax_scale q_i . k_j + bias, bias = -alibi_slopes[h] |i - j|
+ *             or bias_table[bucket_of[clamp(j - i, -D, D) + D], h], D = bias_distance
+ *   out_i = sum_j m[i, j] softmax_j(t) v_j over the visible keys
+ * m = 1, or with dropout the multiplier of g5moe_dropout for the row a = t n_heads + h
+ * (t the query's token index in the packed batch, mod 2^32) and the column j, so that the
+ * mask depends on neither tiles nor launch.  A row whose every term is -inf (bias entries of
+ * -inf) has out = 0 and lse = -inf.  Keys that a query does not see do not enter its sum;
+ * a NaN or infinity in one may still reach the queries that share its 64-key tile, never
+ * another sequence. */
+#define G5MOE_MAX_BIAS_DISTANCE 1024
+typedef struct g5moe_attn_options {
+  int32_t window_left;   /* keys before the query that it sees; -1 = all */
+  int32_t window_right;  /* keys after it; -1 = all */
+  int32_t sink_tokens;   /* first keys of a sequence that every query sees */
+  int32_t bias_buckets;  /* rows of bias_table (0 without one) */
+  int32_t bias_distance; /* D, 1 .. G5MOE_MAX_BIAS_DISTANCE */
+  int32_t bias_dtype;    /* of bias_table and its gradient: G5MOE_DTYPE_BF16 or _F32 */
+  g5moe_dropout dropout; /* of the probabilities; p = 0: none */
+  int32_t reserved;      /* must be 0 */
+} g5moe_attn_options;
+
+/* Forward.  q, k, v, out, cu_seqlens, softmax_scale and shape as in g5moe_attn_varlen_fwd.
+ *   alibi_slopes : fp32 [n_heads] or NULL;  bias_table : [bias_buckets, n_heads] or NULL (at
+ *   most one of the two);  bucket_of : int32 [2 D + 1], each in [0, bias_buckets) (clamped);
+ *   softmax_lse : fp32 [n_heads, total_tokens] out or NULL;  options : NULL = no window, no
+ *   dropout;  ws : g5moe_attn_workspace_size() bytes or NULL, for the key-norm bounds of
+ *   g5moe_attn_varlen_fwd, whose kernel computes the call when it has no window, table or
+ *   dropout (not read otherwise).
+ * Rows of out behind the last sequence are set to 0 (of softmax_lse, left as they were).
+ * Scores, softmax and sums are fp32, the probabilities enter the output product as bf16. */
+g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
+                                  const int32_t* cu_seqlens, const float* alibi_slopes,
+                                  const void* bias_table, const int32_t* bucket_of,
+                                  float softmax_scale, float* softmax_lse, void* ws,
+                                  const g5moe_attn_options* options,
+                                  const g5moe_attn_shape* shape, void* stream);
+
+/* Bytes of workspace g5moe_attn_bwd uses (8 per head and token, 12 with dropout, and with
+ * bias_buckets > 0 the bias sums of every 128-query block). */
+g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
+                                           const g5moe_attn_shape* shape, size_t* bytes);
+
+/* Backward of g5moe_attn_local_fwd and g5moe_attn_varlen_fwd (options NULL), from their out
+ * and softmax_lse and the same inputs, options and seed.
+ *   dout : bf16, the gradient of out;  dq, dk, dv : bf16 out (the gradients of key and value
+ *   heads summed over the query heads that share them);  dbias : [bias_buckets, n_heads] in
+ *   bias_dtype out, or NULL;  ws : g5moe_attn_bwd_workspace_size() bytes, 256-byte aligned;
+ *   grad_shape : shape with the strides of dq, dk, dv and (its o strides) dout.
+ * Rows of dq, dk and dv behind the last sequence are set to 0.  Sums are fp32; P and dS enter
+ * their products as bf16.  No atomics on memory; the order of every sum is fixed. */
+g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                            const void* out, const float* softmax_lse, const int32_t* cu_seqlens,
+                            const float* alibi_slopes, const void* bias_table,
+                            const int32_t* bucket_of, float softmax_scale, void* dq, void* dk,
+                            void* dv, void* dbias, void* ws, const g5moe_attn_options* options,
+                            const g5moe_attn_shape* shape, const g5moe_attn_shape* grad_shape,
+                            void* stream);
+
+/* ---- Residual add with dropout ----------------------------------------------------
+ * out = residual + alpha m x: `hidden_states + dropout(ff_output) * alpha`
+ * (lib/blocks/encoder.py:89), m the multiplier of g5moe_dropout for the row and column of x
+ * (the row in the assignment's place; NULL or p = 0: 1).  x, residual, out : [rows, d] in
+ * dtype (bf16 or fp32), contiguous; out may be x or residual.  One fp32 multiply-add and one
+ * rounding per element.  The backward forms the same mask again: dx = alpha m dout (the
+ * residual's gradient is dout itself). */
+g5moe_status g5moe_dropout_add(const void* x, const void* residual, void* out,
+                               const g5moe_dropout* dropout, float alpha, int64_t rows, int32_t d,
+                               int32_t dtype, void* stream);
+g5moe_status g5moe_dropout_add_backward(const void* dout, void* dx, const g5moe_dropout* dropout,
+                                        float alpha, int64_t rows, int32_t d, int32_t dtype,
+                                        void* stream);
 
 #ifdef __cplusplus
 }
