@@ -923,7 +923,7 @@ static g5moe_status local_args(attn::LocalArgs* a, const int32_t* cu_seqlens,
   a->bucket_of = bucket_of;
   a->bias_bf16 = o.bias_dtype == G5MOE_DTYPE_BF16;
   a->n_buckets = o.bias_buckets;
-  a->far = o.bias_distance;
+  a->far = std::max(0, int(o.bias_distance));
   a->total = s.total_tokens;
   a->max_len = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
   a->q_tok = s.q_token_stride;
@@ -936,6 +936,9 @@ static g5moe_status local_args(attn::LocalArgs* a, const int32_t* cu_seqlens,
   a->o_head = s.o_head_stride;
   return G5MOE_OK;
 }
+
+// Whether ALiBi's leaving out of far keys earns back the pass over the keys' norms.
+static bool use_norms(const attn::LocalArgs& a) { return a.slopes != nullptr && a.max_len > 512; }
 
 g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
                                   const int32_t* cu_seqlens, const float* alibi_slopes,
@@ -975,47 +978,53 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
     return hip_status(e != hipSuccess ? e : attn::launch_zero_behind(a, as_stream(stream)),
                       "g5moe_attn_local_fwd");
   }
+  if (use_norms(a)) a.kmax = static_cast<float*>(ws);
   const bool wide = std::max(s.k_token_stride, s.v_token_stride) >= (int64_t(1) << 24);
   return hip_status(attn::launch_local_fwd(a, wide, as_stream(stream)),
                     "g5moe_attn_local_fwd");
 }
 
-namespace {
-// The backward's workspace: -lse, delta and the dropout row keys per (head, token), the bias
-// sums per workgroup and per distance.
+// The backward's workspace: -lse, delta and the dropout row keys per (head, token); the bias
+// sums per workgroup and per distance; the split sums of dK and dV; the key and query norms.
 struct AttnBwdLayout {
-  size_t nl, delta, rowkey, part, rel, total;
+  size_t nl, delta, rowkey, part, rel, kv_part, sink_part, kmax, qmax, total;
 };
-AttnBwdLayout attn_bwd_layout(const g5moe_attn_options* o, const g5moe_attn_shape& s) {
+static AttnBwdLayout attn_bwd_layout(const attn::LocalArgs& a, const attn::BwdPlan& p) {
   AttnBwdLayout w;
-  const size_t rows = align256(size_t(s.n_heads) * size_t(s.total_tokens) * 4);
   size_t off = 0;
-  w.nl = off;
-  off += rows;
-  w.delta = off;
-  off += rows;
-  w.rowkey = off;
-  if (o != nullptr && o->dropout.p > 0.0f) off += rows;
-  w.part = w.rel = off;
-  if (o != nullptr && o->bias_buckets > 0 && o->bias_distance > 0) {
-    const int top = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
-    off += align256(size_t(attn::bwd_part_floats(top, s.n_seqs, s.n_heads, o->bias_distance)) * 4);
-    w.rel = off;
-    off += align256(size_t(s.n_heads) * size_t(2 * o->bias_distance + 1) * 4);
-  }
+  auto region = [&](int64_t floats) {
+    const size_t at = off;
+    off += align256(size_t(floats) * 4);
+    return at;
+  };
+  const int64_t rows = a.n_heads * a.total;
+  w.nl = region(rows);
+  w.delta = region(rows);
+  w.rowkey = region(a.drop.on ? rows : 0);
+  w.part = region(p.bias_part);
+  w.rel = region(p.bias_part > 0 ? int64_t(a.n_heads) * (2 * a.far + 1) : 0);
+  w.kv_part = region(p.kv_part);
+  w.sink_part = region(p.sink_part);
+  w.kmax = region(int64_t(a.n_heads / a.group) * ((a.total + 63) / 64));
+  w.qmax = region(p.norms);
   w.total = off;
   return w;
 }
-}  // namespace
+static attn::BwdPlan attn_bwd_plan(const attn::LocalArgs& a) {
+  return attn::bwd_plan(a.max_len, a.n_seqs, a.n_heads, a.n_heads / a.group, a.total, a.wl, a.wr,
+                        a.ns, a.far);
+}
 
 g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
                                            const g5moe_attn_shape* shape, size_t* bytes) {
   G5_CHECK(check_attn_shape(shape));
   G5_NONNULL(bytes);
-  if (options != nullptr && options->bias_distance > G5MOE_MAX_BIAS_DISTANCE)
-    return fail(G5MOE_ERR_UNSUPPORTED, "bias_distance %d exceeds %d", int(options->bias_distance),
+  attn::LocalArgs a;
+  G5_CHECK(local_args(&a, nullptr, nullptr, nullptr, nullptr, 0.0f, options, *shape));
+  if (a.far > G5MOE_MAX_BIAS_DISTANCE)
+    return fail(G5MOE_ERR_UNSUPPORTED, "bias_distance %d exceeds %d", a.far,
                 G5MOE_MAX_BIAS_DISTANCE);
-  *bytes = attn_bwd_layout(options, *shape).total;
+  *bytes = a.max_len == 0 || a.n_seqs == 0 ? 0 : attn_bwd_layout(a, attn_bwd_plan(a)).total;
   return G5MOE_OK;
 }
 
@@ -1073,8 +1082,19 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   a.dv_tok = g.v_token_stride;
   a.dv_head = g.v_head_stride;
   a.lse = const_cast<float*>(softmax_lse);
-  const AttnBwdLayout w = attn_bwd_layout(options, s);
+  const attn::BwdPlan plan = attn_bwd_plan(a);
+  const AttnBwdLayout w = attn_bwd_layout(a, plan);
   char* const base = static_cast<char*>(ws);
+  a.q_blocks = plan.q_blocks;
+  a.splits = plan.splits;
+  a.sink_blocks = plan.sink_blocks;
+  a.sink_splits = plan.sink_splits;
+  a.kv_part = reinterpret_cast<float*>(base + w.kv_part);
+  a.sink_part = reinterpret_cast<float*>(base + w.sink_part);
+  if (use_norms(a)) {
+    a.kmax = reinterpret_cast<float*>(base + w.kmax);
+    a.qmax = reinterpret_cast<float*>(base + w.qmax);
+  }
   a.nl = reinterpret_cast<float*>(base + w.nl);
   a.delta = reinterpret_cast<float*>(base + w.delta);
   a.rowkey = reinterpret_cast<uint32_t*>(base + w.rowkey);

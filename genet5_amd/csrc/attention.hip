@@ -80,6 +80,10 @@
 #include "gemm_common.h"
 
 namespace g5moe {
+
+hipError_t launch_key_norm_max(const uint16_t* k, int64_t tok, int64_t head, int64_t total,
+                               int n_heads, float* out, hipStream_t st);
+
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -622,6 +626,14 @@ __global__ __launch_bounds__(256) void key_norm_max_kernel(const uint16_t* __res
 
 }  // namespace
 
+hipError_t launch_key_norm_max(const uint16_t* k, int64_t tok, int64_t head, int64_t total,
+                               int n_heads, float* out, hipStream_t st) {
+  const int n_kblk = int((total + 63) / 64);
+  hipLaunchKernelGGL(key_norm_max_kernel, dim3(unsigned(n_kblk), unsigned(n_heads)), dim3(256), 0,
+                     st, k, tok, head, total, n_kblk, out);
+  return hipGetLastError();
+}
+
 hipError_t launch_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* o,
                            const int32_t* cu_seqlens, const float* slopes, float softmax_scale,
                            float* lse, float* kmax_ws, const g5moe_attn_shape& s,
@@ -643,10 +655,8 @@ hipError_t launch_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t*
                       (slopes != nullptr || s.max_seqlen > 2048);
   const int n_kblk = int((s.total_tokens + 63) / 64);
   if (bounds) {
-    hipLaunchKernelGGL(key_norm_max_kernel, dim3(unsigned(n_kblk), unsigned(s.n_kv_heads)),
-                       dim3(256), 0, st, k, s.k_token_stride, s.k_head_stride, s.total_tokens,
-                       n_kblk, kmax_ws);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = launch_key_norm_max(k, s.k_token_stride, s.k_head_stride, s.total_tokens,
+                                             s.n_kv_heads, kmax_ws, st);
     if (e != hipSuccess) return e;
   }
   AttnArgs a;

@@ -29,10 +29,16 @@ constexpr int kStageQ = 2 * kTileBytes;        // dq_kernel: K tile, V tile
 constexpr int kVecBytes = 1024;                // dkv_kernel: -lse, delta, row keys of a tile
 constexpr int kStageKV = 2 * kTileBytes + kVecBytes;
 
-// A wave's sums of dS by distance live in LDS, one table per half wave: the 32 lanes of a
-// half add to 32 different distances, and a wave's LDS operations keep their order, so the
-// sums do not depend on timing.
-constexpr int kGradTables = 8;
+// A wave adds up dS by distance in a table of its own in LDS, so the order of its sums is
+// fixed.  A 32 x 32 block of dS is first summed along its diagonals: the block goes through
+// LDS (row: query, kDiagPitch floats apart), and lane d of either half wave reads, for its 16
+// queries q, key (q + d) % 32.  Those with q + d < 32 lie on diagonal d, the others on d - 32,
+// so each element is read once; the reads of a step are consecutive, the pitch keeps the
+// 8-byte writes and the reads off each other's banks.  (One LDS float atomic per element
+// instead takes two cycles a lane: 16 x 512 tokens, 12 heads, 193 us for dq_kernel.)
+constexpr int kGradTables = 4;
+constexpr int kDiagPitch = 34;
+constexpr int kDiagFloats = kCols * kDiagPitch;   // per wave
 
 template <int POS, bool DROP, bool DBIAS, bool WIDE>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
@@ -42,6 +48,7 @@ void dq_kernel(LocalArgs a) {
   float* const tab = reinterpret_cast<float*>(smem + kStages * kStageQ);
   const int n_tab = POS == kPosTable ? bias_entries(a.far) : 0;
   float* const gtab = tab + n_tab;
+  float* const diag = gtab + (DBIAS ? kGradTables * n_tab + (n_tab & 1) : 0);  // 8-byte aligned
 
   const int z = blockIdx.z, hq = blockIdx.y;
   if (z == a.n_seqs - 1)
@@ -108,8 +115,21 @@ void dq_kernel(LocalArgs a) {
   BiasChunk bc;
   if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
 
+  // With ALiBi and the key norms, keys farther than `reach` from every query of the workgroup
+  // are left out: P_ij <= 2^(|q||k| sc - sl |i - j| - lse_i log2(e)) < 2^-64 there.
+  int reach = L;
+  if (POS == kPosAlibi && a.kmax != nullptr) {
+    const float qn = norm_max(qf);
+    float v[2] = {qn, own ? nl : -kInf};
+    __shared__ float red[2][4];
+    block_max(v, red, wave, lane);
+    const float bound = __builtin_fabsf(sc) * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
+    reach = alibi_reach(bound + v[1], sl, L);
+    if (tid == 0) a.qmax[(int64_t(hq) * gridDim.z + z) * gridDim.x + blockIdx.x] = v[0];
+  }
   KeyTiles kt;
-  kt.init(q0, min(q0 + kBQ, L) - 1, L, wl, wr, ns);
+  kt.init(q0, min(q0 + kBQ, L) - 1, L, min(wl, reach), min(wr, reach),
+          q0 - (ns - 1) > reach ? 0 : ns);
   TilePair<WIDE> tiles;
   tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
   FragReader fr;
@@ -137,9 +157,8 @@ void dq_kernel(LocalArgs a) {
     const uint32_t span = uint32_t(min(iq + wr, L - 1) - (iq - wl));
     const int sink = ns - j0;
     const float di = float(iq - j0);
-    const int rel0 = j0 - iq + a.far + kBiasPad;
-    const float* tb = tab + rel0;
-    float* gt = gtab + (2 * wave + half) * n_tab + rel0;
+    const float* tb = tab + (j0 - iq + a.far + kBiasPad);
+    float* const dg = diag + wave * kDiagFloats;
     const uint32_t jp = uint32_t(j0) >> 1;
     const float sub = nl + c;
     float sum = 0.0f;
@@ -169,14 +188,28 @@ void dq_kernel(LocalArgs a) {
           d -= delta;
         }
         ds[e] = p * d;
-        if constexpr (DBIAS) {
-          if constexpr (LOOK)
-            __hip_atomic_fetch_add(gt + kr, ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          else
-            sum += ds[e];
-        }
+        if constexpr (DBIAS && !LOOK) sum += ds[e];
       }
+      if constexpr (DBIAS && LOOK)
+        *reinterpret_cast<float2*>(dg + col * kDiagPitch + 8 * (r >> 2) + 4 * half + (r & 3)) =
+            float2{ds[0], ds[1]};
       pk[r >> 1] = pack_bf16x2(ds[0], ds[1]);
+    }
+    if constexpr (DBIAS && LOOK) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      float all = 0.0f, on = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = dg[(16 * half + i) * kDiagPitch + ((16 * half + i + col) & 31)];
+        all += x;
+        on = __builtin_fmaf(x, 16 * half + i + col < 32 ? 1.0f : 0.0f, on);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      all += __shfl_xor(all, 32, 64);
+      on += __shfl_xor(on, 32, 64);
+      // lanes 0 .. 31: diagonal col; lanes 32 .. 63: col - 32
+      gtab[wave * n_tab + (n * kRows + 32 * b - wq + a.far + kBiasPad) + col - 32 * half] +=
+          half == 0 ? on : all - on;
     }
     if constexpr (DBIAS && !LOOK) {
       sum_l += left ? sum : 0.0f;
@@ -303,7 +336,10 @@ void dq_kernel(LocalArgs a) {
   }
 }
 
-// 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).
+// 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).  The
+// tiles of a key block (of each query head that shares the key head) may be split over several
+// workgroups, `splits` of them or `sink_splits` for the blocks that hold sinks, which every
+// query sees: each writes its sums in fp32 and kv_join_kernel adds them up in order.
 template <int POS, bool DROP, bool WIDE>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
 void dkv_kernel(LocalArgs a) {
@@ -318,7 +354,13 @@ void dkv_kernel(LocalArgs a) {
   }
   int s0, L;
   sequence(a, z, s0, L);
-  const int k0 = blockIdx.x * kBQ;
+  // the sinks' blocks first: theirs is the longest work
+  const int n_sink = a.sink_blocks * a.sink_splits;
+  const bool sink_block = int(blockIdx.x) < n_sink;
+  const int splits = sink_block ? a.sink_splits : a.splits;
+  const int bx = sink_block ? int(blockIdx.x) : int(blockIdx.x) - n_sink;
+  const int split = bx % splits;
+  const int k0 = (bx / splits + (sink_block ? 0 : a.sink_blocks)) * kBQ;
   if (k0 >= L) return;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -342,10 +384,33 @@ void dkv_kernel(LocalArgs a) {
     up = a.drop.scale;
   }
 
-  // query tiles that see one of the workgroup's keys
+  // query tiles that see one of the workgroup's keys; with ALiBi and norms not those farther
+  // than `reach` from all of them (lse_i >= -|q||k| sc, the term of key i itself)
+  int reach = L;
+  if (POS == kPosAlibi && a.qmax != nullptr) {
+    __shared__ float red[2][4];
+    float v[1] = {norm_max(kf)};
+    block_max(v, red, wave, lane);
+    reach = 0;
+    for (int g = 0; g < a.group; ++g) {
+      const int h = hk * a.group + g;
+      const float* p = a.qmax + (int64_t(h) * gridDim.z + z) * a.q_blocks;
+      float qn[1] = {0.0f};
+      for (int i = tid; i < (L + kBQ - 1) / kBQ; i += 256) qn[0] = __builtin_fmaxf(qn[0], p[i]);
+      block_max(qn, red, wave, lane);
+      reach = max(reach, alibi_reach(2.0f * __builtin_fabsf(sc) * qn[0] * v[0],
+                                     a.slopes[h] * kLog2e, L));
+    }
+  }
   const int k_hi = min(k0 + kBQ, L) - 1;
-  const int t_lo = k0 < ns ? 0 : max(k0 - wr, 0) / kRows;
-  const int t_hi = k0 < ns ? (L - 1) / kRows : min(k_hi + wl, L - 1) / kRows;
+  const int t_lo = k0 < ns && reach == L ? 0
+                   : max(k0 - min(k0 < ns ? L : wr, reach), 0) / kRows;
+  const int t_hi = min(k_hi + min(k0 < ns ? L : wl, reach), L - 1) / kRows;
+  // this workgroup's share [f, f_end) of (head, tile) in order
+  const int n_t = t_hi - t_lo + 1;
+  const int n_all = n_t * a.group;
+  int f = int(int64_t(n_all) * split / splits);
+  const int f_end = int(int64_t(n_all) * (split + 1) / splits);
 
   TilePair<WIDE> tiles;
   tiles.init(ring, wave, lane, L, a.q_tok * 2, a.do_tok * 2);
@@ -357,8 +422,7 @@ void dkv_kernel(LocalArgs a) {
                             : (DROP && wave == 2) ? reinterpret_cast<const float*>(a.rowkey)
                                                   : a.nl;
   // tiles of (head, number) in order; past the last one it goes out again
-  int h_is = hk * a.group, n_is = t_lo;
-  const int h_end = h_is + a.group;
+  int f_is = f, h_is = hk * a.group + f / n_t, n_is = t_lo + f % n_t;
   auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
     const int h = __builtin_amdgcn_readfirstlane(h_is), n = __builtin_amdgcn_readfirstlane(n_is);
     tiles.issue(reinterpret_cast<const char*>(a.q + int64_t(s0) * a.q_tok + h * a.q_head),
@@ -366,9 +430,11 @@ void dkv_kernel(LocalArgs a) {
                 n, boff);
     gemm::lds_dma4_s(vsrc + int64_t(h) * a.total + s0 + int64_t(n) * kRows,
                      n == tiles.last ? vec_off[1] : vec_off[0], vec_lds + boff);
-    const bool wrap = n_is == t_hi, more = h_is + 1 < h_end;
-    n_is = wrap ? (more ? t_lo : n_is) : n_is + 1;
-    h_is = wrap && more ? h_is + 1 : h_is;
+    if (f_is + 1 < f_end) {
+      ++f_is;
+      h_is += n_is == t_hi ? 1 : 0;
+      n_is = n_is == t_hi ? t_lo : n_is + 1;
+    }
   };
 
   f32x16 dk[2] = {f32x16{}, f32x16{}}, dv[2] = {f32x16{}, f32x16{}};
@@ -447,11 +513,14 @@ void dkv_kernel(LocalArgs a) {
   };
 
   uint32_t boff = 0;
+  if (f < f_end) {
 #pragma unroll
-  for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageKV);
-  gemm::wait_vmcnt<(kStages - 1) * 5>();
-  __syncthreads();
-  for (int h = hk * a.group; h < h_end; ++h) {
+    for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageKV);
+    gemm::wait_vmcnt<(kStages - 1) * 5>();
+    __syncthreads();
+  }
+  while (f < f_end) {
+    const int h = hk * a.group + f / n_t;
     if constexpr (POS == kPosTable) {
       __syncthreads();  // the previous head's table is read no more
       stage_bias(a, h, tab);
@@ -463,7 +532,10 @@ void dkv_kernel(LocalArgs a) {
       sl = a.slopes[h] * kLog2e;
       bc.init(sl, sc, lane);
     }
-    for (int n = t_lo; n <= t_hi; ++n) {
+    const int n_first = t_lo + f % n_t;
+    const int n_last = min(t_hi, n_first + f_end - f - 1);
+    f += n_last - n_first + 1;
+    for (int n = n_first; n <= n_last; ++n) {
       const int i0 = n * kRows, i1 = i0 + kRows - 1;
       const bool some =
           wk < L && ((i0 <= wk_hi + wl && i1 >= wk - wr) || wk < ns);
@@ -533,23 +605,84 @@ void dkv_kernel(LocalArgs a) {
   // refills past the last tile may still be landing in this workgroup's LDS
   gemm::wait_vmcnt<0>();
 
-  if (own) {
-    const int64_t t = s0 + jk;
-    uint16_t* kp = a.dk + t * a.dk_tok + hk * a.dk_head + 4 * half;
-    uint16_t* vp = a.dv + t * a.dv_tok + hk * a.dv_head + 4 * half;
+  if (!own) return;
+  if (splits > 1) {
+    const int64_t row =
+        sink_block ? ((int64_t(z) * a.sink_splits + split) * (a.n_heads / a.group) + hk) *
+                             (a.sink_blocks * kBQ) + jk
+                   : (int64_t(split) * (a.n_heads / a.group) + hk) * a.total + s0 + jk;
+    float* p = (sink_block ? a.sink_part : a.kv_part) + row * (2 * kHeadDim) + 4 * half;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint2 w;
-        w.x = pack_bf16x2(dk[mb][4 * q] * a.scale, dk[mb][4 * q + 1] * a.scale);
-        w.y = pack_bf16x2(dk[mb][4 * q + 2] * a.scale, dk[mb][4 * q + 3] * a.scale);
-        *reinterpret_cast<uint2*>(kp + 32 * mb + 8 * q) = w;
-        w.x = pack_bf16x2(dv[mb][4 * q], dv[mb][4 * q + 1]);
-        w.y = pack_bf16x2(dv[mb][4 * q + 2], dv[mb][4 * q + 3]);
-        *reinterpret_cast<uint2*>(vp + 32 * mb + 8 * q) = w;
+        *reinterpret_cast<f32x4*>(p + 32 * mb + 8 * q) =
+            f32x4{dk[mb][4 * q], dk[mb][4 * q + 1], dk[mb][4 * q + 2], dk[mb][4 * q + 3]};
+        *reinterpret_cast<f32x4*>(p + kHeadDim + 32 * mb + 8 * q) =
+            f32x4{dv[mb][4 * q], dv[mb][4 * q + 1], dv[mb][4 * q + 2], dv[mb][4 * q + 3]};
       }
+    return;
   }
+  const int64_t t = s0 + jk;
+  uint16_t* kp = a.dk + t * a.dk_tok + hk * a.dk_head + 4 * half;
+  uint16_t* vp = a.dv + t * a.dv_tok + hk * a.dv_head + 4 * half;
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint2 w;
+      w.x = pack_bf16x2(dk[mb][4 * q] * a.scale, dk[mb][4 * q + 1] * a.scale);
+      w.y = pack_bf16x2(dk[mb][4 * q + 2] * a.scale, dk[mb][4 * q + 3] * a.scale);
+      *reinterpret_cast<uint2*>(kp + 32 * mb + 8 * q) = w;
+      w.x = pack_bf16x2(dv[mb][4 * q], dv[mb][4 * q + 1]);
+      w.y = pack_bf16x2(dv[mb][4 * q + 2], dv[mb][4 * q + 3]);
+      *reinterpret_cast<uint2*>(vp + 32 * mb + 8 * q) = w;
+    }
+}
+
+// The splits' sums of a key row added up in order.  Rows of the sinks' blocks always where they
+// are split, the others where splits > 1.  32 rows per workgroup, a thread 8 dims of dK and dV.
+__global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a) {
+  const int z = blockIdx.z, hk = blockIdx.y;
+  int s0, L;
+  sequence(a, z, s0, L);
+  const int r = blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int d = 8 * (threadIdx.x & 7);
+  const int sink_rows = a.sink_blocks * kBQ;
+  const bool sink = r < sink_rows;
+  const int splits = sink ? a.sink_splits : a.splits;
+  if (r >= L || splits == 1) return;
+  const int hkv = a.n_heads / a.group;
+  const float* p;
+  int64_t step;
+  if (sink) {
+    step = int64_t(hkv) * sink_rows;
+    p = a.sink_part + (int64_t(z) * splits * step + int64_t(hk) * sink_rows + r) * (2 * kHeadDim);
+  } else {
+    step = int64_t(hkv) * a.total;
+    p = a.kv_part + (int64_t(hk) * a.total + s0 + r) * (2 * kHeadDim);
+  }
+  float k[8] = {}, v[8] = {};
+  for (int i = 0; i < splits; ++i, p += step * (2 * kHeadDim)) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + d + e);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p + kHeadDim + d + e);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        k[e + u] += x[u];
+        v[e + u] += y[u];
+      }
+    }
+  }
+  const int64_t t = s0 + r;
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(k[2 * e] * a.scale, k[2 * e + 1] * a.scale);
+  *reinterpret_cast<u32x4*>(a.dk + t * a.dk_tok + hk * a.dk_head + d) = w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+  *reinterpret_cast<u32x4*>(a.dv + t * a.dv_tok + hk * a.dv_head + d) = w;
 }
 
 // The workgroups' sums by distance added up in order: rel[h, x].  Four waves take every
@@ -600,8 +733,28 @@ __global__ __launch_bounds__(256) void bias_bucket_kernel(LocalArgs a, int E, co
 
 }  // namespace
 
-int64_t bwd_part_floats(int max_seqlen, int n_seqs, int n_heads, int far) {
-  return int64_t((max_seqlen + kBQ - 1) / kBQ) * n_seqs * n_heads * (2 * far + 1);
+// How dkv_kernel's work is split.  Enough workgroups for 256 CUs to hold two each and some to
+// spare, none of less than six tiles; the sinks' blocks into pieces of the other blocks' length.
+BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t total, int wl,
+                 int wr, int ns, int far) {
+  BwdPlan p;
+  p.q_blocks = (max_len + kBQ - 1) / kBQ;
+  const int group = n_heads / n_kv_heads;
+  const int64_t all = int64_t((max_len + kRows - 1) / kRows) * group;
+  const int64_t window = std::min<int64_t>(all, ((int64_t(wl) + wr + kBQ) / kRows + 1) * group);
+  const int64_t blocks = (total / kBQ + n_seqs) * n_kv_heads;
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(1024 / blocks, window / 6)));
+  p.sink_blocks = window < all ? std::min((ns + kBQ - 1) / kBQ, p.q_blocks) : 0;
+  const int64_t piece = std::max<int64_t>(6, window / p.splits);
+  p.sink_splits = p.sink_blocks > 0 ? int(std::min<int64_t>(64, (all + piece - 1) / piece)) : 1;
+  const int64_t row = 2 * kHeadDim;
+  p.kv_part = p.splits > 1 ? int64_t(p.splits) * n_kv_heads * total * row : 0;
+  p.sink_part = p.sink_splits > 1 ? int64_t(n_seqs) * p.sink_splits * n_kv_heads *
+                                        p.sink_blocks * kBQ * row
+                                  : 0;
+  p.bias_part = far > 0 ? int64_t(p.q_blocks) * n_seqs * n_heads * (2 * far + 1) : 0;
+  p.norms = int64_t(p.q_blocks) * n_seqs * n_heads;
+  return p;
 }
 
 hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* rel,
@@ -609,9 +762,12 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
   const unsigned nx = unsigned((a.max_len + kBQ - 1) / kBQ);
   const bool table = a.bias != nullptr, grad = dbias != nullptr;
   const size_t tab = table ? size_t(bias_entries(a.far)) * 4 : 0;
-  const size_t lds_q = size_t(kStages) * kStageQ + tab * (grad ? 1 + kGradTables : 1);
+  const size_t lds_q = size_t(kStages) * kStageQ + tab * (grad ? 1 + kGradTables : 1) +
+                       (grad ? size_t(4) * kDiagFloats * 4 + 8 : 0);
   const size_t lds_kv = size_t(kStages) * kStageKV + tab;
-  auto launch = [&](auto kernel, int heads, size_t lds) {
+  const unsigned kv_x = unsigned(a.sink_blocks * a.sink_splits +
+                                  (int(nx) - a.sink_blocks) * a.splits);
+  auto launch = [&](auto kernel, unsigned x, int heads, size_t lds) {
     // a large max distance needs more than the default limit of 64 KB
     if (lds > 65536 - 2048) {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -619,7 +775,7 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
                                                int(lds));
       if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kernel, dim3(nx, unsigned(heads), unsigned(a.n_seqs)), dim3(256), lds, st,
+    hipLaunchKernelGGL(kernel, dim3(x, unsigned(heads), unsigned(a.n_seqs)), dim3(256), lds, st,
                        a);
     return hipGetLastError();
   };
@@ -629,12 +785,12 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
     constexpr bool D = decltype(drop)::value, W = decltype(w)::value;
     hipError_t e;
     if constexpr (P == kPosTable)
-      e = grad ? launch(dq_kernel<P, D, true, W>, a.n_heads, lds_q)
-               : launch(dq_kernel<P, D, false, W>, a.n_heads, lds_q);
+      e = grad ? launch(dq_kernel<P, D, true, W>, nx, a.n_heads, lds_q)
+               : launch(dq_kernel<P, D, false, W>, nx, a.n_heads, lds_q);
     else
-      e = launch(dq_kernel<P, D, false, W>, a.n_heads, lds_q);
+      e = launch(dq_kernel<P, D, false, W>, nx, a.n_heads, lds_q);
     if (e != hipSuccess) return e;
-    return launch(dkv_kernel<P, D, W>, hkv, lds_kv);
+    return launch(dkv_kernel<P, D, W>, kv_x, hkv, lds_kv);
   };
   using T_ = std::true_type;
   using F_ = std::false_type;
@@ -642,10 +798,23 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
     if (a.drop.on) return wide ? run(pos, T_{}, T_{}) : run(pos, T_{}, F_{});
     return wide ? run(pos, F_{}, T_{}) : run(pos, F_{}, F_{});
   };
+  if (a.kmax != nullptr) {
+    const hipError_t e = launch_key_norm_max(a.k, a.k_tok, a.k_head, a.total, hkv,
+                                             const_cast<float*>(a.kmax), st);
+    if (e != hipSuccess) return e;
+  }
   hipError_t e = table ? pick(std::integral_constant<int, kPosTable>{})
                  : a.slopes != nullptr ? pick(std::integral_constant<int, kPosAlibi>{})
                                        : pick(std::integral_constant<int, kPosNone>{});
-  if (e != hipSuccess || !grad) return e;
+  if (e != hipSuccess) return e;
+  if (a.splits > 1 || (a.sink_blocks > 0 && a.sink_splits > 1)) {
+    const unsigned rows = a.splits > 1 ? nx : unsigned(a.sink_blocks);
+    hipLaunchKernelGGL(kv_join_kernel, dim3(rows * (kBQ / 32), unsigned(hkv), unsigned(a.n_seqs)),
+                       dim3(256), 0, st, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (!grad) return e;
   const int E = 2 * a.far + 1;
   hipLaunchKernelGGL(bias_sum_kernel, dim3(unsigned((E + 63) / 64), unsigned(a.n_heads)),
                      dim3(256), 0, st, a, int(nx), E, rel);

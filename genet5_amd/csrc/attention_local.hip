@@ -76,8 +76,18 @@ void local_fwd_kernel(LocalArgs a) {
     thr = min(a.drop.thr, 65535u) << 16;  // p = 1: the scale is 0
   }
 
+  // With ALiBi and the key norms, keys farther than `reach` from every query of the workgroup
+  // are left out: their probabilities are below 2^-64 of the query's own term, which it sees.
+  int reach = L;
+  if (POS == kPosAlibi && a.kmax != nullptr) {
+    __shared__ float red[2][4];
+    float v[1] = {norm_max(qf)};
+    block_max(v, red, wave, lane);
+    reach = alibi_reach(2.0f * sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane), sl, L);
+  }
   KeyTiles kt;
-  kt.init(q0, min(q0 + kBQ, L) - 1, L, wl, wr, ns);
+  kt.init(q0, min(q0 + kBQ, L) - 1, L, min(wl, reach), min(wr, reach),
+          q0 - (ns - 1) > reach ? 0 : ns);
   TilePair<WIDE> tiles;
   tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
   FragReader fr;
@@ -291,6 +301,11 @@ hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st) {
 hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st) {
   const dim3 grid(unsigned((a.max_len + kBQ - 1) / kBQ), unsigned(a.n_heads),
                   unsigned(a.n_seqs));
+  if (a.kmax != nullptr) {
+    const hipError_t e = launch_key_norm_max(a.k, a.k_tok, a.k_head, a.total,
+                                             a.n_heads / a.group, const_cast<float*>(a.kmax), st);
+    if (e != hipSuccess) return e;
+  }
   const size_t lds =
       size_t(kStages) * kStageBytes + (a.bias != nullptr ? bias_entries(a.far) * 4 : 0);
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a); };

@@ -258,6 +258,15 @@ struct LocalArgs {
   uint32_t* rowkey;                 // backward with dropout: the rows' keys, [n_heads, total]
   float* part;                      // backward: bias sums per workgroup
   int wl, wr, ns;                   // window (large = unlimited), first tokens always visible
+  // with ALiBi, for leaving out tiles whose probabilities vanish, or nullptr: the largest key
+  // norm of each 64-token block [n_kv_heads, ceil(total / 64)], and (backward) the largest
+  // query norm of each 128-query block [n_heads, n_seqs, q_blocks]
+  const float* kmax;
+  float* qmax;
+  int q_blocks;
+  // backward: the splits of a key block's query tiles (of the sinks' blocks) and their sums
+  int splits, sink_blocks, sink_splits;
+  float *kv_part, *sink_part;
   int64_t total;
   int max_len;                      // sequences are not computed past it
   DropoutParams drop;
@@ -269,6 +278,53 @@ __device__ __forceinline__ void sequence(const LocalArgs& a, int z, int& s0, int
   const int total = int(a.total);
   s0 = __builtin_amdgcn_readfirstlane(min(max(a.cu[z], 0), total));
   L = __builtin_amdgcn_readfirstlane(min(min(max(a.cu[z + 1], s0), total) - s0, a.max_len));
+}
+
+// Largest norm of the wave's own 32 rows (every lane).
+__device__ __forceinline__ float norm_max(const bf16x8 (&f)[4]) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(float(f[kc][e]), float(f[kc][e]), ss);
+  ss += __shfl_xor(ss, 32, 64);
+  return __builtin_sqrtf(ss);
+}
+
+// v[i] maximised over the workgroup's 256 lanes.
+template <int N>
+__device__ __forceinline__ void block_max(float (&v)[N], float (*red)[4], int wave, int lane) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int bit = 32; bit >= 1; bit >>= 1) v[i] = __builtin_fmaxf(v[i], __shfl_xor(v[i], bit, 64));
+  __syncthreads();  // red is read no more
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[i][wave] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v[i] = __builtin_fmaxf(__builtin_fmaxf(red[i][0], red[i][1]),
+                           __builtin_fmaxf(red[i][2], red[i][3]));
+}
+
+// Largest key norm over the 64-token blocks that cover a sequence.
+__device__ __forceinline__ float key_norm(const LocalArgs& a, int hk, int s0, int L,
+                                          float (*red)[4], int wave, int lane) {
+  const float* p = a.kmax + int64_t(hk) * ((a.total + 63) / 64);
+  float km[1] = {0.0f};
+  for (int i = (s0 >> 6) + int(threadIdx.x); i <= ((s0 + L - 1) >> 6); i += 256)
+    km[0] = __builtin_fmaxf(km[0], p[i]);
+  block_max(km, red, wave, lane);
+  return km[0];
+}
+
+// The distance from which ALiBi's slope sl (times log2(e)) puts 2^(top - sl distance) below
+// 2^-64; L where there is none (also for an infinite or NaN top).
+__device__ __forceinline__ int alibi_reach(float top, float sl, int L) {
+  const float w = (top + 64.0f) / sl;
+  return __builtin_amdgcn_readfirstlane(sl > 0.0f && w < float(L) ? max(int(w) + 1, 0) : L);
 }
 
 // Rows behind the last sequence, [cu[n_seqs], total), of one head of a bf16 tensor: zeros.
@@ -312,6 +368,12 @@ struct KeyTiles {
   __device__ __forceinline__ int next(int n) const { return n + 1 == s_end ? w_lo : n + 1; }
 };
 
+// The largest norm of each 64-token block of each head of k (attention.hip).
+}  // namespace attn
+hipError_t launch_key_norm_max(const uint16_t* k, int64_t tok, int64_t head, int64_t total,
+                               int n_heads, float* out, hipStream_t st);
+namespace attn {
+
 // Zeros in the rows of out behind the last sequence.
 hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st);
 // wide: a token stride of a streamed matrix of 2^24 elements or more.
@@ -319,8 +381,14 @@ hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st);
 // dbias: [n_buckets, n_heads] out in the table's type, or nullptr; rel: [n_heads, 2 far + 1].
 hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* rel,
                             hipStream_t st);
-// Floats of LocalArgs::part.
-int64_t bwd_part_floats(int max_seqlen, int n_seqs, int n_heads, int far);
+// The splits of the key/value gradients and the floats of the backward's buffers (far: the bias
+// table's largest distance, 0 without a table).
+struct BwdPlan {
+  int q_blocks, splits, sink_blocks, sink_splits;
+  int64_t kv_part, sink_part, bias_part, norms;
+};
+BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t total, int wl,
+                 int wr, int ns, int far);
 
 }  // namespace attn
 }  // namespace g5moe

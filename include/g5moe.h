@@ -650,9 +650,10 @@ typedef struct g5moe_attn_options {
  *   alibi_slopes : fp32 [n_heads] or NULL;  bias_table : [bias_buckets, n_heads] or NULL (at
  *   most one of the two);  bucket_of : int32 [2 D + 1], each in [0, bias_buckets) (clamped);
  *   softmax_lse : fp32 [n_heads, total_tokens] out or NULL;  options : NULL = no window, no
- *   dropout;  ws : g5moe_attn_workspace_size() bytes or NULL, for the key-norm bounds of
- *   g5moe_attn_varlen_fwd, whose kernel computes the call when it has no window, table or
- *   dropout (not read otherwise).
+ *   dropout;  ws : g5moe_attn_workspace_size() bytes or NULL, for the key norms with which
+ *   keys whose probabilities are below 2^-64 of a row's largest under ALiBi are left out, and
+ *   which g5moe_attn_varlen_fwd (whose kernel computes a call without window, table and
+ *   dropout) bounds its terms with.
  * Rows of out behind the last sequence are set to 0 (of softmax_lse, left as they were).
  * Scores, softmax and sums are fp32, the probabilities enter the output product as bf16. */
 g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
@@ -662,8 +663,10 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
                                   const g5moe_attn_options* options,
                                   const g5moe_attn_shape* shape, void* stream);
 
-/* Bytes of workspace g5moe_attn_bwd uses (8 per head and token, 12 with dropout, and with
- * bias_buckets > 0 the bias sums of every 128-query block). */
+/* Bytes of workspace g5moe_attn_bwd uses: 8 per head and token (12 with dropout), with
+ * bias_distance > 0 the bias sums of every 128-query block, fp32 sums of dk and dv where the
+ * query tiles of a key block are split over workgroups, and the norms of key and query
+ * blocks. */
 g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
                                            const g5moe_attn_shape* shape, size_t* bytes);
 

@@ -226,13 +226,23 @@ def test_workspace_size_counts_what_the_backward_keeps(g5lib):
                   ctypes.byref(n))
         return n.value
 
-    rows = 4 * 1000 * 4
-    up = lambda b: (b + 255) // 256 * 256
-    kw = dict(total_tokens=1000, max_seqlen=300, n_seqs=5)
-    assert size(_opts(), **kw) == 2 * up(rows)
-    assert size(_opts(p=0.1), **kw) == 3 * up(rows)
+    # 40,000 tokens keep every workgroup busy without a split
+    up = lambda floats: (floats * 4 + 255) // 256 * 256
+    T, blocks = 40000, 20
+    kw = dict(total_tokens=T, max_seqlen=2500, n_seqs=16, n_heads=8, n_kv_heads=4)
+    base = 2 * up(8 * T) + up(4 * T // 64) + up(blocks * 16 * 8)
+    assert size(_opts(), **kw) == base
+    assert size(_opts(p=0.1), **kw) == base + up(8 * T)
     assert size(_opts(bias_buckets=8, bias_distance=10), **kw) == \
-        2 * up(rows) + up(3 * 5 * 4 * 21 * 4) + up(4 * 21 * 4)
+        base + up(blocks * 16 * 8 * 21) + up(8 * 21)
+    # sinks under a window: their 128 keys' tiles in pieces of the window's length
+    all_tiles, window = 40 * 2, ((100 + 128) // 64 + 1) * 2
+    pieces = -(-all_tiles // window)
+    assert size(_opts(window_left=50, window_right=50, sink_tokens=3), **kw) == \
+        base + up(16 * pieces * 4 * 128 * 128)
+    # few tokens: every key block's tiles are split
+    kw.update(total_tokens=1000, max_seqlen=1000, n_seqs=1)
+    assert size(_opts(), **kw) == 2 * up(8000) + up(4 * 16) + up(8 * 8) + up(5 * 4 * 1000 * 128)
 
 
 @pytest.mark.parametrize("args,match", [
