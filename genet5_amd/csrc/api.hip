@@ -926,6 +926,11 @@ static g5moe_status local_args(attn::LocalArgs* a, const int32_t* cu_seqlens,
   a->far = std::max(0, int(o.bias_distance));
   a->total = s.total_tokens;
   a->max_len = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
+  a->q_blocks = (a->max_len + 127) / 128;
+  // a launch has less than 2^32 work-items, 256 per block
+  if (int64_t(a->q_blocks) * s.n_heads * s.n_seqs > (int64_t(1) << 23))
+    return fail(G5MOE_ERR_UNSUPPORTED, "%d sequences of up to %d tokens and %d heads make more "
+                "than 2^23 blocks of 128 queries", int(s.n_seqs), a->max_len, int(s.n_heads));
   a->q_tok = s.q_token_stride;
   a->k_tok = s.k_token_stride;
   a->v_tok = s.v_token_stride;
@@ -1085,7 +1090,6 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   const attn::BwdPlan plan = attn_bwd_plan(a);
   const AttnBwdLayout w = attn_bwd_layout(a, plan);
   char* const base = static_cast<char*>(ws);
-  a.q_blocks = plan.q_blocks;
   a.splits = plan.splits;
   a.sink_blocks = plan.sink_blocks;
   a.sink_splits = plan.sink_splits;
@@ -1116,9 +1120,8 @@ static g5moe_status dropout_add(const void* x, const void* residual, void* out,
                 int(d));
   if (dtype != G5MOE_DTYPE_BF16 && dtype != G5MOE_DTYPE_F32)
     return fail(G5MOE_ERR_INVALID_ARG, "dtype %d is neither bf16 (0) nor f32 (1)", int(dtype));
-  // one 256-thread workgroup per 256 elements at most, in a grid of 32-bit size
-  if (rows > (int64_t(1) << 38) / d)
-    return fail(G5MOE_ERR_UNSUPPORTED, "%lld rows of %d elements exceed 2^38 elements",
+  if (rows > (int64_t(1) << 40) / d)
+    return fail(G5MOE_ERR_UNSUPPORTED, "%lld rows of %d elements exceed 2^40 elements",
                 (long long)rows, int(d));
   if (rows == 0) return G5MOE_OK;
   G5_NONNULL(x);

@@ -41,7 +41,7 @@ constexpr int kDiagPitch = 34;
 constexpr int kDiagFloats = kCols * kDiagPitch;   // per wave
 
 template <int POS, bool DROP, bool DBIAS, bool WIDE>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(DBIAS || POS == kPosAlibi ? 2 : 3)))
 void dq_kernel(LocalArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   char* const ring = smem;
@@ -50,13 +50,20 @@ void dq_kernel(LocalArgs a) {
   float* const gtab = tab + n_tab;
   float* const diag = gtab + (DBIAS ? kGradTables * n_tab + (n_tab & 1) : 0);  // 8-byte aligned
 
-  const int z = blockIdx.z, hq = blockIdx.y;
-  if (z == a.n_seqs - 1)
-    zero_tail(a, a.dq, a.dq_tok, hq * a.dq_head, int(blockIdx.x), int(gridDim.x));
+  int bx, hq, z;
+  if (!block_of(a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  if (z == a.n_seqs - 1) zero_tail(a, a.dq, a.dq_tok, hq * a.dq_head, bx, a.q_blocks);
   int s0, L;
   sequence(a, z, s0, L);
-  const int q0 = blockIdx.x * kBQ;
-  if (q0 >= L) return;
+  const int q0 = bx * kBQ;
+  if (q0 >= L) {
+    if constexpr (DBIAS) {  // the sums by distance of no query
+      const int E = 2 * a.far + 1;
+      float* out = a.part + ((int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx) * E;
+      for (int x = threadIdx.x; x < E; x += 256) out[x] = 0.0f;
+    }
+    return;
+  }
   const int hk = hq / a.group;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -125,7 +132,7 @@ void dq_kernel(LocalArgs a) {
     block_max(v, red, wave, lane);
     const float bound = __builtin_fabsf(sc) * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
     reach = alibi_reach(bound + v[1], sl, L);
-    if (tid == 0) a.qmax[(int64_t(hq) * gridDim.z + z) * gridDim.x + blockIdx.x] = v[0];
+    if (tid == 0) a.qmax[(int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx] = v[0];
   }
   KeyTiles kt;
   kt.init(q0, min(q0 + kBQ, L) - 1, L, min(wl, reach), min(wr, reach),
@@ -320,8 +327,7 @@ void dq_kernel(LocalArgs a) {
       return v;
     };
     const int E = 2 * a.far + 1;
-    float* out = a.part + (int64_t(hq) * gridDim.z * gridDim.x + int64_t(z) * gridDim.x +
-                           blockIdx.x) * E;
+    float* out = a.part + ((int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx) * E;
     for (int x = tid; x < E; x += 256)
       if (x != 0 && x != E - 1) out[x] = column(kBiasPad + x);
     if (wave < 2) {
@@ -336,6 +342,11 @@ void dq_kernel(LocalArgs a) {
   }
 }
 
+// dkv_kernel's workgroups per head and sequence.
+__host__ __device__ __forceinline__ int kv_blocks(const LocalArgs& a) {
+  return a.sink_blocks * a.sink_splits + (a.q_blocks - a.sink_blocks) * a.splits;
+}
+
 // 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).  The
 // tiles of a key block (of each query head that shares the key head) may be split over several
 // workgroups, `splits` of them or `sink_splits` for the blocks that hold sinks, which every
@@ -347,18 +358,19 @@ void dkv_kernel(LocalArgs a) {
   char* const ring = smem;
   float* const tab = reinterpret_cast<float*>(smem + kStages * kStageKV);
 
-  const int z = blockIdx.z, hk = blockIdx.y;
+  int wx, hk, z;
+  if (!block_of(kv_blocks(a), a.n_heads / a.group, a.n_seqs, wx, hk, z)) return;
   if (z == a.n_seqs - 1) {
-    zero_tail(a, a.dk, a.dk_tok, hk * a.dk_head, int(blockIdx.x), int(gridDim.x));
-    zero_tail(a, a.dv, a.dv_tok, hk * a.dv_head, int(blockIdx.x), int(gridDim.x));
+    zero_tail(a, a.dk, a.dk_tok, hk * a.dk_head, wx, kv_blocks(a));
+    zero_tail(a, a.dv, a.dv_tok, hk * a.dv_head, wx, kv_blocks(a));
   }
   int s0, L;
   sequence(a, z, s0, L);
   // the sinks' blocks first: theirs is the longest work
   const int n_sink = a.sink_blocks * a.sink_splits;
-  const bool sink_block = int(blockIdx.x) < n_sink;
+  const bool sink_block = wx < n_sink;
   const int splits = sink_block ? a.sink_splits : a.splits;
-  const int bx = sink_block ? int(blockIdx.x) : int(blockIdx.x) - n_sink;
+  const int bx = sink_block ? wx : wx - n_sink;
   const int split = bx % splits;
   const int k0 = (bx / splits + (sink_block ? 0 : a.sink_blocks)) * kBQ;
   if (k0 >= L) return;
@@ -394,7 +406,7 @@ void dkv_kernel(LocalArgs a) {
     reach = 0;
     for (int g = 0; g < a.group; ++g) {
       const int h = hk * a.group + g;
-      const float* p = a.qmax + (int64_t(h) * gridDim.z + z) * a.q_blocks;
+      const float* p = a.qmax + (int64_t(h) * a.n_seqs + z) * a.q_blocks;
       float qn[1] = {0.0f};
       for (int i = tid; i < (L + kBQ - 1) / kBQ; i += 256) qn[0] = __builtin_fmaxf(qn[0], p[i]);
       block_max(qn, red, wave, lane);
@@ -685,49 +697,67 @@ __global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a) {
   *reinterpret_cast<u32x4*>(a.dv + t * a.dv_tok + hk * a.dv_head + d) = w;
 }
 
-// The workgroups' sums by distance added up in order: rel[h, x].  Four waves take every
-// fourth workgroup each.
-__global__ __launch_bounds__(256) void bias_sum_kernel(LocalArgs a, int nx, int E, float* rel) {
-  __shared__ float red[4][64];
+// The workgroups' sums by distance added up in order: rel[h, x].  Sixteen waves take every
+// sixteenth of the head's 128-query blocks each (the empty ones wrote zeros), four at a time.
+__global__ __launch_bounds__(1024) void bias_sum_kernel(LocalArgs a, int E, float* rel) {
+  __shared__ float red[16][64];
   const int h = blockIdx.y;
-  const int x = blockIdx.x * 64 + (threadIdx.x & 63);
+  const int lane = threadIdx.x & 63;
+  const int x = blockIdx.x * 64 + lane;
   const int wave = threadIdx.x >> 6;
-  float v = 0.0f;
-  if (x < E)
-    for (int z = 0; z < a.n_seqs; ++z) {
-      int s0, L;
-      sequence(a, z, s0, L);
-      const int nq = min((L + kBQ - 1) / kBQ, nx);
-      const float* p = a.part + ((int64_t(h) * a.n_seqs + z) * nx) * E + x;
-      for (int q = wave; q < nq; q += 4) v += p[int64_t(q) * E];
-    }
-  red[wave][threadIdx.x & 63] = v;
+  float v[4] = {};
+  if (x < E) {
+    const int64_t n = int64_t(a.n_seqs) * a.q_blocks;
+    const float* p = a.part + int64_t(h) * n * E + x;
+    int64_t i = wave;
+    for (; i + 48 < n; i += 64)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] += p[(i + 16 * u) * E];
+    for (; i < n; i += 16) v[0] += p[i * E];
+  }
+  red[wave][lane] = (v[0] + v[1]) + (v[2] + v[3]);
   __syncthreads();
-  if (wave == 0 && x < E)
-    rel[int64_t(h) * E + x] = (red[0][threadIdx.x] + red[1][threadIdx.x]) +
-                              (red[2][threadIdx.x] + red[3][threadIdx.x]);
+  if (wave == 0 && x < E) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += red[w][lane];
+    rel[int64_t(h) * E + x] = sum;
+  }
 }
 
-// dTable[b, h]: the sums of the distances in bucket b, in order.
-__global__ __launch_bounds__(256) void bias_bucket_kernel(LocalArgs a, int E, const float* rel,
-                                                          void* dbias) {
+// dTable[b, h]: the sums of the distances in bucket b, in order: sixteen threads a bucket,
+// each a stretch of the distances.
+__global__ __launch_bounds__(1024) void bias_bucket_kernel(LocalArgs a, int E, const float* rel,
+                                                           void* dbias) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const v = reinterpret_cast<float*>(smem);
   int* const bk = reinterpret_cast<int*>(v + E);
+  __shared__ float red[16][64];
   const int h = blockIdx.x;
-  for (int x = threadIdx.x; x < E; x += 256) {
+  for (int x = threadIdx.x; x < E; x += 1024) {
     v[x] = rel[int64_t(h) * E + x];
     bk[x] = min(max(a.bucket_of[x], 0), a.n_buckets - 1);
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < a.n_buckets; b += 256) {
+  const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int step = (E + 15) / 16;
+  for (int b0 = 0; b0 < a.n_buckets; b0 += 64) {
+    const int b = b0 + lane;
     float sum = 0.0f;
-    for (int x = 0; x < E; ++x) sum += bk[x] == b ? v[x] : 0.0f;
-    const int64_t at = int64_t(b) * a.n_heads + h;
-    if (a.bias_bf16)
-      static_cast<uint16_t*>(dbias)[at] = f32_to_bf16_bits(sum);
-    else
-      static_cast<float*>(dbias)[at] = sum;
+    for (int x = part * step; x < min(E, (part + 1) * step); ++x) sum += bk[x] == b ? v[x] : 0.0f;
+    red[part][lane] = sum;
+    __syncthreads();
+    if (part == 0 && b < a.n_buckets) {
+      sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) sum += red[w][lane];
+      const int64_t at = int64_t(b) * a.n_heads + h;
+      if (a.bias_bf16)
+        static_cast<uint16_t*>(dbias)[at] = f32_to_bf16_bits(sum);
+      else
+        static_cast<float*>(dbias)[at] = sum;
+    }
+    __syncthreads();
   }
 }
 
@@ -743,10 +773,15 @@ BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t t
   const int64_t all = int64_t((max_len + kRows - 1) / kRows) * group;
   const int64_t window = std::min<int64_t>(all, ((int64_t(wl) + wr + kBQ) / kRows + 1) * group);
   const int64_t blocks = (total / kBQ + n_seqs) * n_kv_heads;
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(1024 / blocks, window / 6)));
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(512 / blocks, window / 6)));
   p.sink_blocks = window < all ? std::min((ns + kBQ - 1) / kBQ, p.q_blocks) : 0;
   const int64_t piece = std::max<int64_t>(6, window / p.splits);
-  p.sink_splits = p.sink_blocks > 0 ? int(std::min<int64_t>(64, (all + piece - 1) / piece)) : 1;
+  // (many sequences fill the GPU by themselves, and need no more than 256 MB of sums)
+  const int64_t most = std::max<int64_t>(
+      1, 4096 / (int64_t(n_seqs) * n_kv_heads * std::max(1, p.sink_blocks)));
+  p.sink_splits = p.sink_blocks > 0
+                      ? int(std::min({int64_t(64), most, (all + piece - 1) / piece}))
+                      : 1;
   const int64_t row = 2 * kHeadDim;
   p.kv_part = p.splits > 1 ? int64_t(p.splits) * n_kv_heads * total * row : 0;
   p.sink_part = p.sink_splits > 1 ? int64_t(n_seqs) * p.sink_splits * n_kv_heads *
@@ -759,15 +794,13 @@ BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t t
 
 hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* rel,
                             hipStream_t st) {
-  const unsigned nx = unsigned((a.max_len + kBQ - 1) / kBQ);
+  const int nx = a.q_blocks;
   const bool table = a.bias != nullptr, grad = dbias != nullptr;
   const size_t tab = table ? size_t(bias_entries(a.far)) * 4 : 0;
   const size_t lds_q = size_t(kStages) * kStageQ + tab * (grad ? 1 + kGradTables : 1) +
                        (grad ? size_t(4) * kDiagFloats * 4 + 8 : 0);
   const size_t lds_kv = size_t(kStages) * kStageKV + tab;
-  const unsigned kv_x = unsigned(a.sink_blocks * a.sink_splits +
-                                  (int(nx) - a.sink_blocks) * a.splits);
-  auto launch = [&](auto kernel, unsigned x, int heads, size_t lds) {
+  auto launch = [&](auto kernel, int x, int heads, size_t lds) {
     // a large max distance needs more than the default limit of 64 KB
     if (lds > 65536 - 2048) {
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -775,7 +808,7 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
                                                int(lds));
       if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kernel, dim3(x, unsigned(heads), unsigned(a.n_seqs)), dim3(256), lds, st,
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid_blocks(x, heads, a.n_seqs))), dim3(256), lds, st,
                        a);
     return hipGetLastError();
   };
@@ -790,7 +823,7 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
     else
       e = launch(dq_kernel<P, D, false, W>, nx, a.n_heads, lds_q);
     if (e != hipSuccess) return e;
-    return launch(dkv_kernel<P, D, W>, kv_x, hkv, lds_kv);
+    return launch(dkv_kernel<P, D, W>, kv_blocks(a), hkv, lds_kv);
   };
   using T_ = std::true_type;
   using F_ = std::false_type;
@@ -808,8 +841,8 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
                                        : pick(std::integral_constant<int, kPosNone>{});
   if (e != hipSuccess) return e;
   if (a.splits > 1 || (a.sink_blocks > 0 && a.sink_splits > 1)) {
-    const unsigned rows = a.splits > 1 ? nx : unsigned(a.sink_blocks);
-    hipLaunchKernelGGL(kv_join_kernel, dim3(rows * (kBQ / 32), unsigned(hkv), unsigned(a.n_seqs)),
+    const int rows = a.splits > 1 ? nx : a.sink_blocks;
+    hipLaunchKernelGGL(kv_join_kernel, dim3(unsigned(rows * (kBQ / 32)), unsigned(hkv), unsigned(a.n_seqs)),
                        dim3(256), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -817,11 +850,11 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* r
   if (!grad) return e;
   const int E = 2 * a.far + 1;
   hipLaunchKernelGGL(bias_sum_kernel, dim3(unsigned((E + 63) / 64), unsigned(a.n_heads)),
-                     dim3(256), 0, st, a, int(nx), E, rel);
+                     dim3(1024), 0, st, a, E, rel);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(bias_bucket_kernel, dim3(unsigned(a.n_heads)), dim3(256), size_t(E) * 8, st,
-                     a, E, rel, dbias);
+  hipLaunchKernelGGL(bias_bucket_kernel, dim3(unsigned(a.n_heads)), dim3(1024), size_t(E) * 8,
+                     st, a, E, rel, dbias);
   return hipGetLastError();
 }
 

@@ -31,18 +31,18 @@ constexpr int kBQ = 128;
 constexpr int kStageBytes = 2 * kTileBytes;
 
 template <int POS, bool DROP, bool WIDE>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(3, 3)))
 void local_fwd_kernel(LocalArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   char* const ring = smem;
   float* const tab = reinterpret_cast<float*>(smem + kStages * kStageBytes);
 
-  const int z = blockIdx.z, hq = blockIdx.y;
-  if (z == a.n_seqs - 1)
-    zero_tail(a, a.o, a.o_tok, hq * a.o_head, int(blockIdx.x), int(gridDim.x));
+  int bx, hq, z;
+  if (!block_of(a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  if (z == a.n_seqs - 1) zero_tail(a, a.o, a.o_tok, hq * a.o_head, bx, a.q_blocks);
   int s0, L;
   sequence(a, z, s0, L);
-  const int q0 = blockIdx.x * kBQ;
+  const int q0 = bx * kBQ;
   if (q0 >= L) return;
   const int hk = hq / a.group;
   const int tid = threadIdx.x;
@@ -104,19 +104,10 @@ void local_fwd_kernel(LocalArgs a) {
     tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff);
     n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
   };
-  bf16x8 kf[2][4];
-  auto load_kf = [&](uint32_t boff) __attribute__((always_inline)) {
-#pragma unroll
-    for (int kc = 0; kc < 4; ++kc)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) kf[b][kc] = fr.row(ring + boff, b, kc);
-  };
-
   f32x16 o[2] = {f32x16{}, f32x16{}};
   float m = -kInf, psum = 0.0f;
   float ms = 0.0f;  // what the exponents subtract: m, or 0 while every term was -inf
   f32x16 s[2];
-  uint32_t pk[2][8];
 
   auto advance = [&](float mx) __attribute__((always_inline)) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
@@ -134,9 +125,9 @@ void local_fwd_kernel(LocalArgs a) {
         for (int r = 0; r < 16; ++r) o[mb][r] *= alpha;
     }
   };
-  // The probabilities of the scores in s, tile n.  c: the tile's constant bias (neither MASK
-  // nor LOOK: added here; else part of the terms already).
-  auto softmax = [&](auto plain_c, int n, float c) __attribute__((always_inline)) {
+  // The softmax step of the scores in s (PLAIN: scores to be scaled, the tile's constant bias c
+  // to be added; else terms) and the output product, 32 keys at a time.
+  auto step = [&](auto plain_c, int n, float c, const char* V) __attribute__((always_inline)) {
     constexpr bool PLAIN = decltype(plain_c)::value;
     float mx = s[0][0];
 #pragma unroll
@@ -152,7 +143,8 @@ void local_fwd_kernel(LocalArgs a) {
     const uint32_t jp = uint32_t(n * kRows + 4 * half) >> 1;
     float sum = 0.0f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b) {
+      uint32_t pk[8];
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         float p[2];
@@ -168,8 +160,17 @@ void local_fwd_kernel(LocalArgs a) {
           p[0] = (bits << 16) >= thr ? p[0] : 0.0f;
           p[1] = bits >= thr ? p[1] : 0.0f;
         }
-        pk[b][r >> 1] = pack_bf16x2(p[0], p[1]);
+        pk[r >> 1] = pack_bf16x2(p[0], p[1]);
       }
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc) {
+        const bf16x8 pf = chunk(pk, cc);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+          o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.trans(V, 2 * b + cc, mb), pf, o[mb],
+                                                          0, 0, 0);
+      }
+    }
     psum += sum;
   };
   // Per-element terms in place of the scores.
@@ -205,24 +206,20 @@ void local_fwd_kernel(LocalArgs a) {
   for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageBytes);
   gemm::wait_vmcnt<(kStages - 1) * 4>();
   __syncthreads();
-  load_kf(0);
   for (; count > 0; --count, n = kt.next(n)) {
     const int j0 = n * kRows, j1 = j0 + kRows - 1;
     // what the wave's queries see of the tile
     const bool some = wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
-    bf16x8 vf[4][2];
     if (some) {
       const f32x16 zero16 = {};
+      const char* const K = ring + boff;
+      const char* const V = K + kTileBytes;
 #pragma unroll
       for (int kc = 0; kc < 4; ++kc)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][kc], qf[kc],
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(K, b, kc), qf[kc],
                                                          kc == 0 ? zero16 : s[b], 0, 0, 0);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb) vf[c][mb] = fr.trans(ring + boff + kTileBytes, c, mb);
       const bool all = j1 < L && ((j0 >= wq_hi - wl && j1 <= wq + wr) || j1 < ns);
       using T_ = std::true_type;
       using F_ = std::false_type;
@@ -239,7 +236,7 @@ void local_fwd_kernel(LocalArgs a) {
         if (!look) bc.add(s, float(iq - j0), before);
       }
       if (all && !look) {
-        softmax(T_{}, n, c);
+        step(T_{}, n, c, V);
       } else {
         if (POS == kPosNone || !look)
           terms(T_{}, F_{}, n, c);
@@ -247,7 +244,7 @@ void local_fwd_kernel(LocalArgs a) {
           terms(F_{}, T_{}, n, c);
         else
           terms(T_{}, T_{}, n, c);
-        softmax(F_{}, n, c);
+        step(F_{}, n, c, V);
       }
     }
     // the next stage landed, and every wave has read all of this one
@@ -255,16 +252,6 @@ void local_fwd_kernel(LocalArgs a) {
     __syncthreads();
     issue(boff);
     boff = boff + kStageBytes == kStages * kStageBytes ? 0 : boff + kStageBytes;
-    load_kf(boff);
-    if (some) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bf16x8 pf = chunk(pk[c >> 1], c & 1);
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
-          o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[c][mb], pf, o[mb], 0, 0, 0);
-      }
-    }
   }
   // refills past the last tile may still be landing in this workgroup's LDS
   gemm::wait_vmcnt<0>();
@@ -299,8 +286,7 @@ hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st) {
-  const dim3 grid(unsigned((a.max_len + kBQ - 1) / kBQ), unsigned(a.n_heads),
-                  unsigned(a.n_seqs));
+  const dim3 grid(unsigned(grid_blocks(a.q_blocks, a.n_heads, a.n_seqs)));
   if (a.kmax != nullptr) {
     const hipError_t e = launch_key_norm_max(a.k, a.k_tok, a.k_head, a.total,
                                              a.n_heads / a.group, const_cast<float*>(a.kmax), st);

@@ -272,6 +272,27 @@ struct LocalArgs {
   DropoutParams drop;
 };
 
+// The workgroup's (x, head, sequence) of nx x heads x sequences, from a one-dimensional grid of
+// grid_blocks() workgroups: consecutive workgroups go to the eight XCDs in turn, so runs of
+// kRun blocks x of one head are given to one XCD, whose L2 then serves their common tiles.
+// False: nothing to do.
+constexpr int kXcds = 8;
+constexpr int kRun = 8;
+__device__ __forceinline__ bool block_of(int nx, int heads, int n_seqs, int& x, int& h, int& z) {
+  const uint32_t id = blockIdx.x;
+  const uint32_t j = id / kXcds;
+  const uint32_t item = ((j / kRun) * kXcds + id % kXcds) * kRun + j % kRun;
+  const uint32_t pair = item / uint32_t(nx);
+  x = int(item % uint32_t(nx));
+  h = int(pair % uint32_t(heads));
+  z = int(pair / uint32_t(heads));
+  return z < n_seqs;
+}
+inline int64_t grid_blocks(int64_t nx, int64_t heads, int64_t n_seqs) {
+  constexpr int64_t unit = kXcds * kRun;
+  return (nx * heads * n_seqs + unit - 1) / unit * unit;
+}
+
 // Sequence z's first token and length, clamped to [0, total] and max_len: a malformed
 // cu_seqlens cannot move an access outside the buffers.
 __device__ __forceinline__ void sequence(const LocalArgs& a, int z, int& s0, int& L) {

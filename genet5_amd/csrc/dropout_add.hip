@@ -7,6 +7,8 @@
 // What bounds it: memory, two reads and one write (one and one in the backward) per element;
 // a thread moves 16 bytes of each operand, and its hashes (one per two elements, two for the
 // row) are hidden behind the loads.
+#include <algorithm>
+
 #include "g5moe_internal.h"
 
 namespace g5moe {
@@ -57,32 +59,34 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ 
                                                           uint32_t per_row, float up,
                                                           DropoutParams drop) {
   constexpr int N = VEC ? Vec<T>::kN : 1;
-  const int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (u >= pieces) return;
-  // 32-bit division where the numbers allow it
-  const int64_t row = pieces <= int64_t(UINT32_MAX) ? int64_t(uint32_t(u) / per_row) : u / per_row;
-  const uint32_t c0 = uint32_t(u - row * per_row) * N;
-  const uint32_t key = dropout_row_key(uint32_t(row), drop.seed_lo, drop.seed_hi);
-  if constexpr (VEC) {
-    float v[N], r[N];
-    Vec<T>::load(v, x + u * N);
-    if constexpr (ADD) Vec<T>::load(r, residual + u * N);
+  for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < pieces;
+       u += int64_t(gridDim.x) * 256) {
+    // 32-bit division where the numbers allow it
+    const int64_t row =
+        pieces <= int64_t(UINT32_MAX) ? int64_t(uint32_t(u) / per_row) : u / per_row;
+    const uint32_t c0 = uint32_t(u - row * per_row) * N;
+    const uint32_t key = dropout_row_key(uint32_t(row), drop.seed_lo, drop.seed_hi);
+    if constexpr (VEC) {
+      float v[N], r[N];
+      Vec<T>::load(v, x + u * N);
+      if constexpr (ADD) Vec<T>::load(r, residual + u * N);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint32_t bits = dropout_pair_bits(key, (c0 + i) >> 1);
+      for (int i = 0; i < N; i += 2) {
+        const uint32_t bits = dropout_pair_bits(key, (c0 + i) >> 1);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool keep = (e == 0 ? bits & 0xffffu : bits >> 16) >= drop.thr;
-        const float base = ADD ? r[i + e] : 0.0f;
-        v[i + e] = keep ? __builtin_fmaf(v[i + e], up, base) : base;
+        for (int e = 0; e < 2; ++e) {
+          const bool keep = (e == 0 ? bits & 0xffffu : bits >> 16) >= drop.thr;
+          const float base = ADD ? r[i + e] : 0.0f;
+          v[i + e] = keep ? __builtin_fmaf(v[i + e], up, base) : base;
+        }
       }
+      Vec<T>::store(out + u * N, v);
+    } else {
+      const uint32_t bits = dropout_pair_bits(key, c0 >> 1);
+      const bool keep = ((c0 & 1) ? bits >> 16 : bits & 0xffffu) >= drop.thr;
+      const float base = ADD ? Vec<T>::get(residual + u) : 0.0f;
+      Vec<T>::put(out + u, keep ? __builtin_fmaf(Vec<T>::get(x + u), up, base) : base);
     }
-    Vec<T>::store(out + u * N, v);
-  } else {
-    const uint32_t bits = dropout_pair_bits(key, c0 >> 1);
-    const bool keep = ((c0 & 1) ? bits >> 16 : bits & 0xffffu) >= drop.thr;
-    const float base = ADD ? Vec<T>::get(residual + u) : 0.0f;
-    Vec<T>::put(out + u, keep ? __builtin_fmaf(Vec<T>::get(x + u), up, base) : base);
   }
 }
 
@@ -95,7 +99,8 @@ hipError_t launch(const void* x, const void* residual, void* out, int64_t rows, 
   const int per_row = vec ? d / Vec<T>::kN : d;
   const int64_t pieces = rows * per_row;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned((pieces + 255) / 256)), dim3(256), 0, st,
+    hipLaunchKernelGGL(kernel, dim3(unsigned(std::min<int64_t>((pieces + 255) / 256, 1 << 20))),
+                       dim3(256), 0, st,
                        static_cast<const T*>(x), static_cast<const T*>(residual),
                        static_cast<T*>(out), pieces, uint32_t(per_row), up, drop);
     return hipGetLastError();

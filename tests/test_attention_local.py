@@ -248,7 +248,7 @@ def test_workspace_size_counts_what_the_backward_keeps(g5lib):
 @pytest.mark.parametrize("args,match", [
     (dict(p=1.5), "dropout.p"), (dict(d=0), "d 0"), (dict(rows=-1), "rows"),
     (dict(dtype=3), "dtype"), (dict(x=None), "x is NULL"), (dict(out=None), "out is NULL"),
-    (dict(residual=None), "residual is NULL"), (dict(rows=1 << 40), "exceed"),
+    (dict(residual=None), "residual is NULL"), (dict(rows=1 << 42), "exceed"),
 ])
 def test_dropout_add_c_refusals(g5lib, args, match):
     a = dict(x=FAKE, residual=FAKE, out=FAKE, p=0.1, rows=4, d=8, dtype=0)
