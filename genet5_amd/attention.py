@@ -264,11 +264,13 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                    alibi_slopes: Optional[torch.Tensor] = None,
                    relative_bias: Optional[torch.Tensor] = None, max_distance: int = 128,
                    window_size: Tuple[int, int] = (-1, -1), sink_tokens: int = 0,
-                   dropout_p: float = 0.0, dropout_seed: int = 0, return_lse: bool = False):
+                   dropout_p: float = 0.0, dropout_seed: int = 0, return_lse: bool = False,
+                   return_norms: bool = False):
     """g5moe_attn_local_fwd on the current stream: attention over the visible keys with an
     optional position bias and dropout.  Tensors as attn_varlen_fwd takes them;
     relative_bias [num_buckets, H] bf16 or fp32.  Returns out [T, H, 64] (and softmax_lse
-    [H, T] fp32 when return_lse); rows behind the last sequence are zeros in out."""
+    [H, T] fp32 when return_lse, and with return_norms what attn_bwd takes as key_norms);
+    rows behind the last sequence are zeros in out."""
     dev = _check_device(q)
     T, H = q.shape[0], q.shape[1]
     Hkv = k.shape[1] if k.dim() == 3 else -1
@@ -299,6 +301,8 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                  _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias), _ptr(buckets),
                  ctypes.c_float(softmax_scale), _ptr(lse), _ptr(ws), ctypes.byref(opts),
                  ctypes.byref(shape), _stream(dev))
+    if return_norms:
+        return out, lse, ws if alibi_slopes is not None and not empty else None
     return (out, lse) if return_lse else out
 
 
@@ -308,10 +312,13 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
              alibi_slopes: Optional[torch.Tensor] = None,
              relative_bias: Optional[torch.Tensor] = None, max_distance: int = 128,
              window_size: Tuple[int, int] = (-1, -1), sink_tokens: int = 0,
-             dropout_p: float = 0.0, dropout_seed: int = 0, bias_grad: bool = True):
+             dropout_p: float = 0.0, dropout_seed: int = 0, bias_grad: bool = True,
+             key_norms: Optional[torch.Tensor] = None):
     """g5moe_attn_bwd on the current stream: (dq, dk, dv, d_relative_bias) of a forward with
     these arguments, from its out and softmax_lse; d_relative_bias is None without a table
-    or with bias_grad = False.  Rows behind the last sequence are zeros."""
+    or with bias_grad = False.  key_norms: the forward's (attn_local_fwd, return_norms), which
+    the call would otherwise form again under ALiBi.  Rows behind the last sequence are
+    zeros."""
     dev = _check_device(q)
     T, H = q.shape[0], q.shape[1]
     Hkv = k.shape[1] if k.dim() == 3 else -1
@@ -349,7 +356,7 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     ops._call_on(dev, "g5moe_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                  _ptr(softmax_lse), _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias),
                  _ptr(buckets), ctypes.c_float(softmax_scale), _ptr(dq), _ptr(dk), _ptr(dv),
-                 _ptr(dbias), _ptr(ws), ctypes.byref(opts), ctypes.byref(shape),
+                 _ptr(dbias), _ptr(key_norms), _ptr(ws), ctypes.byref(opts), ctypes.byref(shape),
                  ctypes.byref(gshape), _stream(dev))
     return dq, dk, dv, dbias
 
@@ -359,7 +366,7 @@ def _draw_seed() -> int:
     return int(torch.randint(0, 2 ** 62, (1,)).item())
 
 
-def _bwd_call(need_bias, dout, q, k, v, out, lse, cu, slopes, bias, call, seed):
+def _bwd_call(need_bias, dout, q, k, v, out, lse, cu, slopes, bias, norms, call, seed):
     """attn_bwd with dout brought into a form the kernel reads."""
     max_seqlen, scale, max_distance, wl, wr, sinks, p = call
     st = dout.stride()
@@ -367,7 +374,7 @@ def _bwd_call(need_bias, dout, q, k, v, out, lse, cu, slopes, bias, call, seed):
             or dout.data_ptr() % 16:
         dout = dout.to(torch.bfloat16).contiguous()
     return attn_bwd(dout, q, k, v, out, lse, cu, max_seqlen, scale, slopes, bias, max_distance,
-                    (wl, wr), sinks, p, seed, need_bias)
+                    (wl, wr), sinks, p, seed, need_bias, norms)
 
 
 class _AttnFunction(torch.autograd.Function):
@@ -377,9 +384,10 @@ class _AttnFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, cu, max_seqlen, scale, slopes, max_distance, wl, wr, sinks,
                 p, seed):
-        out, lse = attn_local_fwd(q, k, v, cu, max_seqlen, scale, slopes, bias, max_distance,
-                                  (wl, wr), sinks, p, seed, return_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, cu, slopes, bias)
+        out, lse, norms = attn_local_fwd(q, k, v, cu, max_seqlen, scale, slopes, bias,
+                                         max_distance, (wl, wr), sinks, p, seed, return_lse=True,
+                                         return_norms=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu, slopes, bias, norms)
         ctx.call = (max_seqlen, scale, max_distance, wl, wr, sinks, p)
         ctx.seed = seed
         ctx.mark_non_differentiable(lse)
@@ -434,7 +442,7 @@ def _attn_local_bwd_op(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv, d_relative_bias or an empty tensor)."""
     dq, dk, dv, db = _bwd_call(bias_grad, dout, q, k, v, out, lse, cu_seqlens, alibi_slopes,
-                               relative_bias, (max_seqlen, softmax_scale, max_distance,
+                               relative_bias, None, (max_seqlen, softmax_scale, max_distance,
                                                window_left, window_right, sink_tokens,
                                                dropout_p), int(seed[0]))
     return dq, dk, dv, q.new_empty((0,)) if db is None else db

@@ -926,9 +926,8 @@ static g5moe_status local_args(attn::LocalArgs* a, const int32_t* cu_seqlens,
   a->far = std::max(0, int(o.bias_distance));
   a->total = s.total_tokens;
   a->max_len = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
-  a->q_blocks = (a->max_len + 127) / 128;
   // a launch has less than 2^32 work-items, 256 per block
-  if (int64_t(a->q_blocks) * s.n_heads * s.n_seqs > (int64_t(1) << 23))
+  if (int64_t((a->max_len + 127) / 128) * s.n_heads * s.n_seqs > (int64_t(1) << 23))
     return fail(G5MOE_ERR_UNSUPPORTED, "%d sequences of up to %d tokens and %d heads make more "
                 "than 2^23 blocks of 128 queries", int(s.n_seqs), a->max_len, int(s.n_heads));
   a->q_tok = s.q_token_stride;
@@ -985,14 +984,17 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
   }
   if (use_norms(a)) a.kmax = static_cast<float*>(ws);
   const bool wide = std::max(s.k_token_stride, s.v_token_stride) >= (int64_t(1) << 24);
+  a.ks = attn::pick_ks((s.total_tokens / 128 + s.n_seqs) * s.n_heads);
+  a.q_rows = 128 / a.ks;
+  a.q_blocks = (a.max_len + a.q_rows - 1) / a.q_rows;
   return hip_status(attn::launch_local_fwd(a, wide, as_stream(stream)),
                     "g5moe_attn_local_fwd");
 }
 
 // The backward's workspace: -lse, delta and the dropout row keys per (head, token); the bias
-// sums per workgroup and per distance; the split sums of dK and dV; the key and query norms.
+// sums per workgroup; the split sums of dK and dV; the key and query norms.
 struct AttnBwdLayout {
-  size_t nl, delta, rowkey, part, rel, kv_part, sink_part, kmax, qmax, total;
+  size_t nl, delta, rowkey, part, kv_part, sink_part, kmax, qmax, total;
 };
 static AttnBwdLayout attn_bwd_layout(const attn::LocalArgs& a, const attn::BwdPlan& p) {
   AttnBwdLayout w;
@@ -1007,7 +1009,6 @@ static AttnBwdLayout attn_bwd_layout(const attn::LocalArgs& a, const attn::BwdPl
   w.delta = region(rows);
   w.rowkey = region(a.drop.on ? rows : 0);
   w.part = region(p.bias_part);
-  w.rel = region(p.bias_part > 0 ? int64_t(a.n_heads) * (2 * a.far + 1) : 0);
   w.kv_part = region(p.kv_part);
   w.sink_part = region(p.sink_part);
   w.kmax = region(int64_t(a.n_heads / a.group) * ((a.total + 63) / 64));
@@ -1037,9 +1038,9 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
                             const void* out, const float* softmax_lse, const int32_t* cu_seqlens,
                             const float* alibi_slopes, const void* bias_table,
                             const int32_t* bucket_of, float softmax_scale, void* dq, void* dk,
-                            void* dv, void* dbias, void* ws, const g5moe_attn_options* options,
-                            const g5moe_attn_shape* shape, const g5moe_attn_shape* grad_shape,
-                            void* stream) {
+                            void* dv, void* dbias, const float* key_norms, void* ws,
+                            const g5moe_attn_options* options, const g5moe_attn_shape* shape,
+                            const g5moe_attn_shape* grad_shape, void* stream) {
   G5_CHECK(check_attn_shape(shape));
   G5_CHECK(check_attn_shape(grad_shape));
   const g5moe_attn_shape& s = *shape;
@@ -1087,25 +1088,31 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   a.dv_tok = g.v_token_stride;
   a.dv_head = g.v_head_stride;
   a.lse = const_cast<float*>(softmax_lse);
+  const bool wide = std::max({s.q_token_stride, s.k_token_stride, s.v_token_stride,
+                              g.o_token_stride}) >= (int64_t(1) << 24);
   const attn::BwdPlan plan = attn_bwd_plan(a);
   const AttnBwdLayout w = attn_bwd_layout(a, plan);
   char* const base = static_cast<char*>(ws);
+  a.ks = plan.ks;
+  a.q_rows = 128 / plan.ks;
+  a.q_blocks = plan.q_blocks;
+  a.kv_ks = plan.kv_ks;
+  a.kv_blocks = plan.kv_blocks;
   a.splits = plan.splits;
   a.sink_blocks = plan.sink_blocks;
   a.sink_splits = plan.sink_splits;
   a.kv_part = reinterpret_cast<float*>(base + w.kv_part);
   a.sink_part = reinterpret_cast<float*>(base + w.sink_part);
   if (use_norms(a)) {
-    a.kmax = reinterpret_cast<float*>(base + w.kmax);
+    a.kmax = key_norms != nullptr ? key_norms : reinterpret_cast<float*>(base + w.kmax);
     a.qmax = reinterpret_cast<float*>(base + w.qmax);
   }
+  a.dbias = dbias;
   a.nl = reinterpret_cast<float*>(base + w.nl);
   a.delta = reinterpret_cast<float*>(base + w.delta);
   a.rowkey = reinterpret_cast<uint32_t*>(base + w.rowkey);
   a.part = reinterpret_cast<float*>(base + w.part);
-  const bool wide = std::max({s.q_token_stride, s.k_token_stride, s.v_token_stride,
-                              g.o_token_stride}) >= (int64_t(1) << 24);
-  return hip_status(attn::launch_local_bwd(a, wide, dbias, reinterpret_cast<float*>(base + w.rel),
+  return hip_status(attn::launch_local_bwd(a, wide, a.kmax != nullptr && key_norms == nullptr,
                                            as_stream(stream)),
                     "g5moe_attn_bwd");
 }

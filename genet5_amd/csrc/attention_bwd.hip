@@ -24,10 +24,9 @@ namespace g5moe {
 namespace attn {
 namespace {
 
-constexpr int kBQ = 128;                       // own rows per workgroup, both kernels
-constexpr int kStageQ = 2 * kTileBytes;        // dq_kernel: K tile, V tile
+constexpr int kPairQ = 2 * kTileBytes;         // dq_kernel: K tile, V tile
 constexpr int kVecBytes = 1024;                // dkv_kernel: -lse, delta, row keys of a tile
-constexpr int kStageKV = 2 * kTileBytes + kVecBytes;
+constexpr int kPairKV = 2 * kTileBytes + kVecBytes;
 
 // A wave adds up dS by distance in a table of its own in LDS, so the order of its sums is
 // fixed.  A 32 x 32 block of dS is first summed along its diagonals: the block goes through
@@ -40,22 +39,26 @@ constexpr int kGradTables = 4;
 constexpr int kDiagPitch = 34;
 constexpr int kDiagFloats = kCols * kDiagPitch;   // per wave
 
-template <int POS, bool DROP, bool DBIAS, bool WIDE>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(DBIAS || POS == kPosAlibi ? 2 : 3)))
+template <int POS, bool DROP, bool DBIAS, bool WIDE, int KS>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
 void dq_kernel(LocalArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  using S = Split<KS>;
+  constexpr int kStageQ = KS * kPairQ;
   char* const ring = smem;
-  float* const tab = reinterpret_cast<float*>(smem + kStages * kStageQ);
+  float* const tab = reinterpret_cast<float*>(smem + S::kStages * kStageQ);
   const int n_tab = POS == kPosTable ? bias_entries(a.far) : 0;
   float* const gtab = tab + n_tab;
   float* const diag = gtab + (DBIAS ? kGradTables * n_tab + (n_tab & 1) : 0);  // 8-byte aligned
 
   int bx, hq, z;
-  if (!block_of(a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  if (!block_of(blockIdx.x, a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  if (POS == kPosAlibi && a.kmax != nullptr && a.n_heads <= 64)
+    by_slope(a.slopes, a.n_heads, a.n_seqs, hq, z);
   if (z == a.n_seqs - 1) zero_tail(a, a.dq, a.dq_tok, hq * a.dq_head, bx, a.q_blocks);
   int s0, L;
   sequence(a, z, s0, L);
-  const int q0 = bx * kBQ;
+  const int q0 = bx * S::kOwn;
   if (q0 >= L) {
     if constexpr (DBIAS) {  // the sums by distance of no query
       const int E = 2 * a.far + 1;
@@ -69,7 +72,8 @@ void dq_kernel(LocalArgs a) {
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int wq = q0 + wave * kCols;
+  const int tg = S::tile(wave);
+  const int wq = q0 + S::own(wave) * kCols;
   const int wq_hi = min(wq + kCols, L) - 1;
   const int iq = wq + col;
   const bool own = iq < L;
@@ -78,65 +82,16 @@ void dq_kernel(LocalArgs a) {
   const float sl = POS == kPosAlibi ? a.slopes[hq] * kLog2e : 0.0f;
 
   bf16x8 qf[4], dof[4];
-  float delta = 0.0f, nl = -kInf;  // a row past the end has probabilities of 0
+  OwnRows qr, dor, orw;
+  float lse;
   {
     const int64_t t = s0 + min(iq, L - 1);
-    load_own(qf, a.q + t * a.q_tok + hq * a.q_head, half, own, 0u);
-    load_own(dof, a.dout + t * a.do_tok + hq * a.do_head, half, own, 0u);
-    bf16x8 of[4];
-    load_own(of, a.o + t * a.o_tok + hq * a.o_head, half, own, 0u);
-#pragma unroll
-    for (int kc = 0; kc < 4; ++kc)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        delta = __builtin_fmaf(float(dof[kc][e]), float(of[kc][e]), delta);
-    delta += __shfl_xor(delta, 32, 64);
-    const int64_t at = int64_t(hq) * a.total + t;
-    if (own) {
-      const float lse = a.lse[at];
-      // an empty row: every term is -inf, whatever is subtracted
-      nl = lse == -kInf ? 0.0f : -lse * kLog2e;
-    }
-    asm volatile("" : "+v"(nl));
-  }
-  uint32_t rkey = 0, thr = 0;
-  float up = 0.0f;
-  if constexpr (DROP) {
-    rkey = dropout_row_key(uint32_t(s0 + iq) * uint32_t(a.n_heads) + uint32_t(hq),
-                           a.drop.seed_lo, a.drop.seed_hi);
-    thr = min(a.drop.thr, 65535u) << 16;  // p = 1: the scale is 0
-    up = a.drop.scale;
-  }
-  if (own && half == 0) {
-    const int64_t at = int64_t(hq) * a.total + s0 + iq;
-    a.nl[at] = nl;
-    a.delta[at] = delta;
-    if constexpr (DROP) a.rowkey[at] = rkey;
-  }
-  if constexpr (POS == kPosTable) stage_bias(a, hq, tab);
-  if constexpr (DBIAS)
-    for (int x = tid; x < kGradTables * n_tab; x += 256) gtab[x] = 0.0f;
-  if constexpr (POS == kPosTable) __syncthreads();
-  const float far_l = POS == kPosTable ? tab[0] : 0.0f;
-  const float far_r = POS == kPosTable ? tab[n_tab - 1] : 0.0f;
-  BiasChunk bc;
-  if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
-
-  // With ALiBi and the key norms, keys farther than `reach` from every query of the workgroup
-  // are left out: P_ij <= 2^(|q||k| sc - sl |i - j| - lse_i log2(e)) < 2^-64 there.
-  int reach = L;
-  if (POS == kPosAlibi && a.kmax != nullptr) {
-    const float qn = norm_max(qf);
-    float v[2] = {qn, own ? nl : -kInf};
-    __shared__ float red[2][4];
-    block_max(v, red, wave, lane);
-    const float bound = __builtin_fabsf(sc) * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
-    reach = alibi_reach(bound + v[1], sl, L);
-    if (tid == 0) a.qmax[(int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx] = v[0];
+    qr.request(a.q + t * a.q_tok + hq * a.q_head, half);
+    lse = a.lse[int64_t(hq) * a.total + t];
+    dor.request(a.dout + t * a.do_tok + hq * a.do_head, half);
+    orw.request(a.o + t * a.o_tok + hq * a.o_head, half);
   }
   KeyTiles kt;
-  kt.init(q0, min(q0 + kBQ, L) - 1, L, min(wl, reach), min(wr, reach),
-          q0 - (ns - 1) > reach ? 0 : ns);
   TilePair<WIDE> tiles;
   tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
   FragReader fr;
@@ -146,11 +101,69 @@ void dq_kernel(LocalArgs a) {
   const char* const vbase =
       reinterpret_cast<const char*>(a.v + int64_t(s0) * a.v_tok + hk * a.v_head);
   // past the last tile it goes out again, into a buffer that no later tile reads
-  int n_is = kt.first();
+  int n_is = 0;
   auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
-    tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff);
-    n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
+#pragma unroll
+    for (int g = 0; g < KS; ++g) {
+      tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff + g * kPairQ);
+      n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
+    }
   };
+  auto begin = [&](int reach) __attribute__((always_inline)) {
+    kt.init(q0, min(q0 + S::kOwn, L) - 1, L, min(wl, reach), min(wr, reach),
+            q0 - (ns - 1) > reach ? 0 : ns);
+    n_is = kt.first();
+#pragma unroll
+    for (int st = 0; st < S::kStages; ++st) issue(uint32_t(st) * kStageQ);
+  };
+  if constexpr (POS != kPosAlibi) begin(L);
+  qr.take(qf, own, 0u);
+  // a row past the end has probabilities of 0; of an empty row every term is -inf, whatever
+  // is subtracted
+  float nl = !own ? -kInf : lse == -kInf ? 0.0f : -lse * kLog2e;
+  asm volatile("" : "+v"(nl));
+  if constexpr (POS == kPosAlibi) {
+    // With the key norms, keys farther than `reach` from every query of the workgroup are left
+    // out: P_ij <= 2^(|q||k| sc - sl |i - j| - lse_i log2(e)) < 2^-64 there.
+    int reach = L;
+    if (a.kmax != nullptr) {
+      float v[2] = {norm_max(qf), nl};
+      __shared__ float red[2][4];
+      block_max(v, red, wave, lane);
+      const float bound = __builtin_fabsf(sc) * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
+      reach = alibi_reach(bound + v[1], sl, L);
+      if (tid == 0) a.qmax[(int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx] = v[0];
+    }
+    begin(reach);
+  }
+  dor.take(dof, own, 0u);
+  float delta = 0.0f;
+  {
+    bf16x8 of[4];
+    orw.take(of, own, 0u);
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        delta = __builtin_fmaf(float(dof[kc][e]), float(of[kc][e]), delta);
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  uint32_t rkey = 0, thr = 0;
+  float up = 0.0f;
+  if constexpr (DROP) {
+    rkey = dropout_row_key(uint32_t(s0 + iq) * uint32_t(a.n_heads) + uint32_t(hq),
+                           a.drop.seed_lo, a.drop.seed_hi);
+    thr = min(a.drop.thr, 65535u) << 16;  // p = 1: the scale is 0
+    up = a.drop.scale;
+  }
+  if constexpr (POS == kPosTable) stage_bias(a, hq, tab);
+  if constexpr (DBIAS)
+    for (int x = tid; x < kGradTables * n_tab; x += 256) gtab[x] = 0.0f;
+  if constexpr (POS == kPosTable) __syncthreads();
+  const float far_l = POS == kPosTable ? tab[0] : 0.0f;
+  const float far_r = POS == kPosTable ? tab[n_tab - 1] : 0.0f;
+  BiasChunk bc;
+  if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
 
   f32x16 dq[2] = {f32x16{}, f32x16{}};
   float sum_l = 0.0f, sum_r = 0.0f;  // dS at distances <= -far and >= far in plain tiles
@@ -224,29 +237,28 @@ void dq_kernel(LocalArgs a) {
     }
   };
 
-  int count = kt.s_end + kt.w_hi - kt.w_lo + 1;
   int n = kt.first();
+  if (tg == 1) n = kt.next(n);
   uint32_t boff = 0;
-#pragma unroll
-  for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageQ);
-  gemm::wait_vmcnt<(kStages - 1) * 4>();
+  gemm::wait_vmcnt<(S::kStages - 1) * 4 * KS>();
   __syncthreads();
-  for (; count > 0; --count, n = kt.next(n)) {
+  for (int left = kt.count(); left > 0; left -= KS) {
     const int j0 = n * kRows, j1 = j0 + kRows - 1;
-    const bool some = wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
+    const bool some =
+        left > tg && wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
     if (some) {
       const f32x16 zero16 = {};
-      const char* const K = ring + boff;
+      const char* const K = ring + boff + tg * kPairQ;
       const char* const V = K + kTileBytes;
       const bool all = j1 < L && ((j0 >= wq_hi - wl && j1 <= wq + wr) || j1 < ns);
       using T_ = std::true_type;
       using F_ = std::false_type;
       float c = 0.0f;
-      bool look = false, left = false, before = false;
+      bool look = false, far_left = false, before = false;
       if constexpr (POS == kPosTable) {
-        left = j1 - wq <= -a.far;
-        look = !left && j0 - wq_hi < a.far;
-        c = left ? far_l : far_r;
+        far_left = j1 - wq <= -a.far;
+        look = !far_left && j0 - wq_hi < a.far;
+        c = far_left ? far_l : far_r;
       }
       if constexpr (POS == kPosAlibi) {
         before = j1 <= wq;
@@ -273,9 +285,9 @@ void dq_kernel(LocalArgs a) {
             grad(T_{}, T_{}, n, b, s, dp, 0.0f, false, pk);
         } else {
           if (all)
-            grad(F_{}, F_{}, n, b, s, dp, c, left, pk);
+            grad(F_{}, F_{}, n, b, s, dp, c, far_left, pk);
           else
-            grad(T_{}, F_{}, n, b, s, dp, c, left, pk);
+            grad(T_{}, F_{}, n, b, s, dp, c, far_left, pk);
         }
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
@@ -288,15 +300,38 @@ void dq_kernel(LocalArgs a) {
       }
     }
     // the next stage landed, and every wave has read all of this one
-    gemm::wait_vmcnt<(kStages - 2) * 4>();
+    gemm::wait_vmcnt<(S::kStages - 2) * 4 * KS>();
     __syncthreads();
     issue(boff);
-    boff = boff + kStageQ == kStages * kStageQ ? 0 : boff + kStageQ;
+    boff = boff + kStageQ == S::kStages * kStageQ ? 0 : boff + kStageQ;
+#pragma unroll
+    for (int g = 0; g < KS; ++g) n = kt.next(n);
   }
   // refills past the last tile may still be landing in this workgroup's LDS
   gemm::wait_vmcnt<0>();
 
-  if (own) {
+  if (own && half == 0 && tg == 0) {  // for dkv_kernel
+    const int64_t at = int64_t(hq) * a.total + s0 + iq;
+    a.nl[at] = nl;
+    a.delta[at] = delta;
+    if constexpr (DROP) a.rowkey[at] = rkey;
+  }
+  bool holds = true;
+  if constexpr (KS == 2) {
+    float v[32];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      v[r] = dq[0][r];
+      v[16 + r] = dq[1][r];
+    }
+    holds = join_waves(v, ring, wave, lane);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dq[0][r] = v[r];
+      dq[1][r] = v[16 + r];
+    }
+  }
+  if (own && holds) {
     uint16_t* op = a.dq + int64_t(s0 + iq) * a.dq_tok + hq * a.dq_head + 4 * half;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
@@ -342,24 +377,70 @@ void dq_kernel(LocalArgs a) {
   }
 }
 
+// The gradient of one head's column of the bias table, by one workgroup: the sums by distance
+// of dq_kernel's workgroups added up in order (empty ones wrote zeros), then those of each
+// bucket.  E distances, a thread per distance and (up to 256) stretch of the workgroups.
+__device__ __forceinline__ void bias_grad(const LocalArgs& a, int h, float* rel) {
+  const int E = 2 * a.far + 1;
+  const int64_t n = int64_t(a.n_seqs) * a.q_blocks;
+  const float* const p = a.part + int64_t(h) * n * E;
+  for (int x = threadIdx.x; x < E; x += 256) {
+    float v[8] = {};
+    int64_t i = 0;
+    for (; i + 8 <= n; i += 8)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] += p[(i + u) * E + x];
+    for (; i < n; ++i) v[0] += p[i * E + x];
+    rel[x] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+  }
+  int* const bucket = reinterpret_cast<int*>(rel + E);
+  for (int x = threadIdx.x; x < E; x += 256)
+    bucket[x] = min(max(a.bucket_of[x], 0), a.n_buckets - 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.n_buckets; b += 256) {
+    float sum = 0.0f;
+    for (int x = 0; x < E; ++x) sum += bucket[x] == b ? rel[x] : 0.0f;
+    const int64_t at = int64_t(b) * a.n_heads + h;
+    if (a.bias_bf16)
+      static_cast<uint16_t*>(a.dbias)[at] = f32_to_bf16_bits(sum);
+    else
+      static_cast<float*>(a.dbias)[at] = sum;
+  }
+}
+
 // dkv_kernel's workgroups per head and sequence.
 __host__ __device__ __forceinline__ int kv_blocks(const LocalArgs& a) {
-  return a.sink_blocks * a.sink_splits + (a.q_blocks - a.sink_blocks) * a.splits;
+  return a.sink_blocks * a.sink_splits + (a.kv_blocks - a.sink_blocks) * a.splits;
 }
 
 // 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).  The
 // tiles of a key block (of each query head that shares the key head) may be split over several
 // workgroups, `splits` of them or `sink_splits` for the blocks that hold sinks, which every
 // query sees: each writes its sums in fp32 and kv_join_kernel adds them up in order.
-template <int POS, bool DROP, bool WIDE>
+template <int POS, bool DROP, bool WIDE, int KS>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
 void dkv_kernel(LocalArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  using S = Split<KS>;
+  constexpr int kStageKV = KS * kPairKV;
   char* const ring = smem;
-  float* const tab = reinterpret_cast<float*>(smem + kStages * kStageKV);
+  float* const tab = reinterpret_cast<float*>(smem + S::kStages * kStageKV);
 
+  // the first workgroups reduce the bias gradient, behind which the others' work hides
+  uint32_t id = blockIdx.x;
+  if constexpr (POS == kPosTable) {
+    if (a.dbias != nullptr) {
+      if (id < uint32_t(a.n_heads)) {
+        bias_grad(a, int(id), reinterpret_cast<float*>(smem));
+        return;
+      }
+      id -= uint32_t(a.n_heads);
+    }
+  }
   int wx, hk, z;
-  if (!block_of(kv_blocks(a), a.n_heads / a.group, a.n_seqs, wx, hk, z)) return;
+  if (!block_of(id, kv_blocks(a), a.n_heads / a.group, a.n_seqs, wx, hk, z)) return;
+  if (POS == kPosAlibi && a.qmax != nullptr && a.group == 1 && a.n_heads <= 64)
+    by_slope(a.slopes, a.n_heads, a.n_seqs, hk, z);
   if (z == a.n_seqs - 1) {
     zero_tail(a, a.dk, a.dk_tok, hk * a.dk_head, wx, kv_blocks(a));
     zero_tail(a, a.dv, a.dv_tok, hk * a.dv_head, wx, kv_blocks(a));
@@ -372,13 +453,14 @@ void dkv_kernel(LocalArgs a) {
   const int splits = sink_block ? a.sink_splits : a.splits;
   const int bx = sink_block ? wx : wx - n_sink;
   const int split = bx % splits;
-  const int k0 = (bx / splits + (sink_block ? 0 : a.sink_blocks)) * kBQ;
+  const int k0 = (bx / splits + (sink_block ? 0 : a.sink_blocks)) * S::kOwn;
   if (k0 >= L) return;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int wk = k0 + wave * kCols;               // the wave's keys: wk .. wk_hi
+  const int tg = S::tile(wave);
+  const int wk = k0 + S::own(wave) * kCols;               // the wave's keys: wk .. wk_hi
   const int wk_hi = min(wk + kCols, L) - 1;
   const int jk = wk + col;
   const bool own = jk < L;
@@ -386,8 +468,9 @@ void dkv_kernel(LocalArgs a) {
   const float sc = a.sc;
 
   bf16x8 kf[4], vf[4];
-  load_own(kf, a.k + int64_t(s0 + min(jk, L - 1)) * a.k_tok + hk * a.k_head, half, own, 0u);
-  load_own(vf, a.v + int64_t(s0 + min(jk, L - 1)) * a.v_tok + hk * a.v_head, half, own, 0u);
+  OwnRows kr, vr;
+  kr.request(a.k + int64_t(s0 + min(jk, L - 1)) * a.k_tok + hk * a.k_head, half);
+  vr.request(a.v + int64_t(s0 + min(jk, L - 1)) * a.v_tok + hk * a.v_head, half);
   uint32_t thr = 0, golden_c = 0;
   float up = 0.0f;
   if constexpr (DROP) {
@@ -395,6 +478,7 @@ void dkv_kernel(LocalArgs a) {
     golden_c = (uint32_t(jk) >> 1) * 0x9e3779b9u;
     up = a.drop.scale;
   }
+  if constexpr (POS == kPosAlibi) kr.take(kf, own, 0u);
 
   // query tiles that see one of the workgroup's keys; with ALiBi and norms not those farther
   // than `reach` from all of them (lse_i >= -|q||k| sc, the term of key i itself)
@@ -408,21 +492,24 @@ void dkv_kernel(LocalArgs a) {
       const int h = hk * a.group + g;
       const float* p = a.qmax + (int64_t(h) * a.n_seqs + z) * a.q_blocks;
       float qn[1] = {0.0f};
-      for (int i = tid; i < (L + kBQ - 1) / kBQ; i += 256) qn[0] = __builtin_fmaxf(qn[0], p[i]);
+      for (int i = tid; i < (L + a.q_rows - 1) / a.q_rows; i += 256) qn[0] = __builtin_fmaxf(qn[0], p[i]);
       block_max(qn, red, wave, lane);
       reach = max(reach, alibi_reach(2.0f * __builtin_fabsf(sc) * qn[0] * v[0],
                                      a.slopes[h] * kLog2e, L));
     }
   }
-  const int k_hi = min(k0 + kBQ, L) - 1;
+  const int k_hi = min(k0 + S::kOwn, L) - 1;
   const int t_lo = k0 < ns && reach == L ? 0
                    : max(k0 - min(k0 < ns ? L : wr, reach), 0) / kRows;
   const int t_hi = min(k_hi + min(k0 < ns ? L : wl, reach), L - 1) / kRows;
-  // this workgroup's share [f, f_end) of (head, tile) in order
+  // this workgroup's share of (head, tile) in order: (h_a, n_a) .. (h_b, n_b)
   const int n_t = t_hi - t_lo + 1;
   const int n_all = n_t * a.group;
-  int f = int(int64_t(n_all) * split / splits);
-  const int f_end = int(int64_t(n_all) * (split + 1) / splits);
+  const int f_a = int(int64_t(n_all) * split / splits);
+  const int f_b = int(int64_t(n_all) * (split + 1) / splits) - 1;
+  const bool work = f_a <= f_b;
+  const int h_a = hk * a.group + f_a / n_t, n_a = t_lo + f_a % n_t;
+  const int h_b = hk * a.group + f_b / n_t, n_b = t_lo + f_b % n_t;
 
   TilePair<WIDE> tiles;
   tiles.init(ring, wave, lane, L, a.q_tok * 2, a.do_tok * 2);
@@ -433,19 +520,26 @@ void dkv_kernel(LocalArgs a) {
   const float* const vsrc = wave == 1 ? a.delta
                             : (DROP && wave == 2) ? reinterpret_cast<const float*>(a.rowkey)
                                                   : a.nl;
-  // tiles of (head, number) in order; past the last one it goes out again
-  int f_is = f, h_is = hk * a.group + f / n_t, n_is = t_lo + f % n_t;
+  // KS tiles of one head at a time, the last of a head's repeated where there is none left;
+  // past the last step it goes out again
+  int h_is = h_a, n_is = n_a, n_stop = h_a == h_b ? n_b : t_hi;
   auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
-    const int h = __builtin_amdgcn_readfirstlane(h_is), n = __builtin_amdgcn_readfirstlane(n_is);
-    tiles.issue(reinterpret_cast<const char*>(a.q + int64_t(s0) * a.q_tok + h * a.q_head),
-                reinterpret_cast<const char*>(a.dout + int64_t(s0) * a.do_tok + h * a.do_head),
-                n, boff);
-    gemm::lds_dma4_s(vsrc + int64_t(h) * a.total + s0 + int64_t(n) * kRows,
-                     n == tiles.last ? vec_off[1] : vec_off[0], vec_lds + boff);
-    if (f_is + 1 < f_end) {
-      ++f_is;
-      h_is += n_is == t_hi ? 1 : 0;
-      n_is = n_is == t_hi ? t_lo : n_is + 1;
+#pragma unroll
+    for (int g = 0; g < KS; ++g) {
+      const int h = __builtin_amdgcn_readfirstlane(h_is);
+      const int n = __builtin_amdgcn_readfirstlane(min(n_is + g, n_stop));
+      tiles.issue(reinterpret_cast<const char*>(a.q + int64_t(s0) * a.q_tok + h * a.q_head),
+                  reinterpret_cast<const char*>(a.dout + int64_t(s0) * a.do_tok + h * a.do_head),
+                  n, boff + g * kPairKV);
+      gemm::lds_dma4_s(vsrc + int64_t(h) * a.total + s0 + int64_t(n) * kRows,
+                       n == tiles.last ? vec_off[1] : vec_off[0], vec_lds + boff + g * kPairKV);
+    }
+    if (n_is + KS <= n_stop) {
+      n_is += KS;
+    } else if (h_is < h_b) {
+      ++h_is;
+      n_is = t_lo;
+      n_stop = h_is == h_b ? n_b : t_hi;
     }
   };
 
@@ -455,7 +549,7 @@ void dkv_kernel(LocalArgs a) {
 
   // P (dropped) and dS of 32 queries: half b of tile n, scores s and dP dp.
   auto grad = [&](auto mask_c, auto look_c, int n, int b, const f32x16& s, const f32x16& dp,
-                  float c, uint32_t boff, uint32_t (&pkp)[8], uint32_t (&pkd)[8])
+                  float c, uint32_t pair, uint32_t (&pkp)[8], uint32_t (&pkd)[8])
       __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_c)::value, LOOK = decltype(look_c)::value;
     const int i0 = n * kRows + 32 * b + 4 * half;
@@ -468,7 +562,7 @@ void dkv_kernel(LocalArgs a) {
     const float dj = float(jk - i0);
     const float* tb = tab + (jk - i0 - 31 + a.far + kBiasPad);
     const float* vec =
-        reinterpret_cast<const float*>(ring + boff + 2 * kTileBytes) + 32 * b + 4 * half;
+        reinterpret_cast<const float*>(ring + pair + 2 * kTileBytes) + 32 * b + 4 * half;
     uint32_t hb[8];
     if constexpr (DROP) {
       // a pair of lanes being the two columns of one hash, even lanes hash for the first 16
@@ -524,15 +618,18 @@ void dkv_kernel(LocalArgs a) {
     }
   };
 
-  uint32_t boff = 0;
-  if (f < f_end) {
+  if (work) {
 #pragma unroll
-    for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageKV);
-    gemm::wait_vmcnt<(kStages - 1) * 5>();
+    for (int st = 0; st < S::kStages; ++st) issue(uint32_t(st) * kStageKV);
+  }
+  if constexpr (POS != kPosAlibi) kr.take(kf, own, 0u);
+  vr.take(vf, own, 0u);
+  uint32_t boff = 0;
+  if (work) {
+    gemm::wait_vmcnt<(S::kStages - 1) * 5 * KS>();
     __syncthreads();
   }
-  while (f < f_end) {
-    const int h = hk * a.group + f / n_t;
+  for (int h = h_a; work && h <= h_b; ++h) {
     if constexpr (POS == kPosTable) {
       __syncthreads();  // the previous head's table is read no more
       stage_bias(a, h, tab);
@@ -544,16 +641,16 @@ void dkv_kernel(LocalArgs a) {
       sl = a.slopes[h] * kLog2e;
       bc.init(sl, sc, lane);
     }
-    const int n_first = t_lo + f % n_t;
-    const int n_last = min(t_hi, n_first + f_end - f - 1);
-    f += n_last - n_first + 1;
-    for (int n = n_first; n <= n_last; ++n) {
+    const int n_last = h == h_b ? n_b : t_hi;
+    for (int first = h == h_a ? n_a : t_lo; first <= n_last; first += KS) {
+      const int n = first + tg;
       const int i0 = n * kRows, i1 = i0 + kRows - 1;
       const bool some =
-          wk < L && ((i0 <= wk_hi + wl && i1 >= wk - wr) || wk < ns);
+          n <= n_last && wk < L && ((i0 <= wk_hi + wl && i1 >= wk - wr) || wk < ns);
       if (some) {
         const f32x16 zero16 = {};
-        const char* const Q = ring + boff;
+        const uint32_t pair = boff + tg * kPairKV;
+        const char* const Q = ring + pair;
         const char* const D = Q + kTileBytes;
         const bool all = i1 < L && ((i1 <= wk + wl && i0 >= wk_hi - wr) || wk_hi < ns);
         using T_ = std::true_type;
@@ -585,14 +682,14 @@ void dkv_kernel(LocalArgs a) {
             if (!look) s = bc.add_half(s, b, float(jk - i0), before);
           if (POS != kPosNone && look) {
             if (all)
-              grad(F_{}, T_{}, n, b, s, dp, 0.0f, boff, pkp, pkd);
+              grad(F_{}, T_{}, n, b, s, dp, 0.0f, pair, pkp, pkd);
             else
-              grad(T_{}, T_{}, n, b, s, dp, 0.0f, boff, pkp, pkd);
+              grad(T_{}, T_{}, n, b, s, dp, 0.0f, pair, pkp, pkd);
           } else {
             if (all)
-              grad(F_{}, F_{}, n, b, s, dp, c, boff, pkp, pkd);
+              grad(F_{}, F_{}, n, b, s, dp, c, pair, pkp, pkd);
             else
-              grad(T_{}, F_{}, n, b, s, dp, c, boff, pkp, pkd);
+              grad(T_{}, F_{}, n, b, s, dp, c, pair, pkp, pkd);
           }
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
@@ -608,20 +705,38 @@ void dkv_kernel(LocalArgs a) {
         }
       }
       // the next stage landed, and every wave has read all of this one
-      gemm::wait_vmcnt<(kStages - 2) * 5>();
+      gemm::wait_vmcnt<(S::kStages - 2) * 5 * KS>();
       __syncthreads();
       issue(boff);
-      boff = boff + kStageKV == kStages * kStageKV ? 0 : boff + kStageKV;
+      boff = boff + kStageKV == S::kStages * kStageKV ? 0 : boff + kStageKV;
     }
   }
   // refills past the last tile may still be landing in this workgroup's LDS
   gemm::wait_vmcnt<0>();
 
+  if constexpr (KS == 2) {
+    float v[64];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        v[32 * i + r] = dk[i][r];
+        v[32 * i + 16 + r] = dv[i][r];
+      }
+    if (!join_waves(v, ring, wave, lane)) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dk[i][r] = v[32 * i + r];
+        dv[i][r] = v[32 * i + 16 + r];
+      }
+  }
   if (!own) return;
   if (splits > 1) {
     const int64_t row =
         sink_block ? ((int64_t(z) * a.sink_splits + split) * (a.n_heads / a.group) + hk) *
-                             (a.sink_blocks * kBQ) + jk
+                             (a.sink_blocks * S::kOwn) + jk
                    : (int64_t(split) * (a.n_heads / a.group) + hk) * a.total + s0 + jk;
     float* p = (sink_block ? a.sink_part : a.kv_part) + row * (2 * kHeadDim) + 4 * half;
 #pragma unroll
@@ -660,7 +775,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a) {
   sequence(a, z, s0, L);
   const int r = blockIdx.x * 32 + (threadIdx.x >> 3);
   const int d = 8 * (threadIdx.x & 7);
-  const int sink_rows = a.sink_blocks * kBQ;
+  const int sink_rows = a.sink_blocks * (128 / a.kv_ks);
   const bool sink = r < sink_rows;
   const int splits = sink ? a.sink_splits : a.splits;
   if (r >= L || splits == 1) return;
@@ -697,84 +812,29 @@ __global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a) {
   *reinterpret_cast<u32x4*>(a.dv + t * a.dv_tok + hk * a.dv_head + d) = w;
 }
 
-// The workgroups' sums by distance added up in order: rel[h, x].  Sixteen waves take every
-// sixteenth of the head's 128-query blocks each (the empty ones wrote zeros), four at a time.
-__global__ __launch_bounds__(1024) void bias_sum_kernel(LocalArgs a, int E, float* rel) {
-  __shared__ float red[16][64];
-  const int h = blockIdx.y;
-  const int lane = threadIdx.x & 63;
-  const int x = blockIdx.x * 64 + lane;
-  const int wave = threadIdx.x >> 6;
-  float v[4] = {};
-  if (x < E) {
-    const int64_t n = int64_t(a.n_seqs) * a.q_blocks;
-    const float* p = a.part + int64_t(h) * n * E + x;
-    int64_t i = wave;
-    for (; i + 48 < n; i += 64)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] += p[(i + 16 * u) * E];
-    for (; i < n; i += 16) v[0] += p[i * E];
-  }
-  red[wave][lane] = (v[0] + v[1]) + (v[2] + v[3]);
-  __syncthreads();
-  if (wave == 0 && x < E) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) sum += red[w][lane];
-    rel[int64_t(h) * E + x] = sum;
-  }
-}
-
-// dTable[b, h]: the sums of the distances in bucket b, in order: sixteen threads a bucket,
-// each a stretch of the distances.
-__global__ __launch_bounds__(1024) void bias_bucket_kernel(LocalArgs a, int E, const float* rel,
-                                                           void* dbias) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* const v = reinterpret_cast<float*>(smem);
-  int* const bk = reinterpret_cast<int*>(v + E);
-  __shared__ float red[16][64];
-  const int h = blockIdx.x;
-  for (int x = threadIdx.x; x < E; x += 1024) {
-    v[x] = rel[int64_t(h) * E + x];
-    bk[x] = min(max(a.bucket_of[x], 0), a.n_buckets - 1);
-  }
-  __syncthreads();
-  const int part = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int step = (E + 15) / 16;
-  for (int b0 = 0; b0 < a.n_buckets; b0 += 64) {
-    const int b = b0 + lane;
-    float sum = 0.0f;
-    for (int x = part * step; x < min(E, (part + 1) * step); ++x) sum += bk[x] == b ? v[x] : 0.0f;
-    red[part][lane] = sum;
-    __syncthreads();
-    if (part == 0 && b < a.n_buckets) {
-      sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) sum += red[w][lane];
-      const int64_t at = int64_t(b) * a.n_heads + h;
-      if (a.bias_bf16)
-        static_cast<uint16_t*>(dbias)[at] = f32_to_bf16_bits(sum);
-      else
-        static_cast<float*>(dbias)[at] = sum;
-    }
-    __syncthreads();
-  }
-}
-
 }  // namespace
 
-// How dkv_kernel's work is split.  Enough workgroups for 256 CUs to hold two each and some to
-// spare, none of less than six tiles; the sinks' blocks into pieces of the other blocks' length.
+// How the backward's work is split: enough workgroups for 256 CUs to hold two each and some to
+// spare, none of less than six steps; the sinks' key blocks into pieces of the others' length.
 BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t total, int wl,
                  int wr, int ns, int far) {
   BwdPlan p;
-  p.q_blocks = (max_len + kBQ - 1) / kBQ;
+  const int64_t full = total / 128 + n_seqs;  // blocks of 128 rows of one head, about
+  // (with a table's sums in LDS beside two KS = 2 stages a CU would hold one workgroup)
+  p.ks = far > 0 ? 1 : pick_ks(full * n_heads);
+  const int q_rows = 128 / p.ks;
+  p.q_blocks = (max_len + q_rows - 1) / q_rows;
   const int group = n_heads / n_kv_heads;
-  const int64_t all = int64_t((max_len + kRows - 1) / kRows) * group;
-  const int64_t window = std::min<int64_t>(all, ((int64_t(wl) + wr + kBQ) / kRows + 1) * group);
-  const int64_t blocks = (total / kBQ + n_seqs) * n_kv_heads;
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(512 / blocks, window / 6)));
-  p.sink_blocks = window < all ? std::min((ns + kBQ - 1) / kBQ, p.q_blocks) : 0;
+  p.kv_ks = pick_ks(full * n_kv_heads);
+  const int kv_rows = 128 / p.kv_ks;
+  p.kv_blocks = (max_len + kv_rows - 1) / kv_rows;
+  // steps of a workgroup that holds 64 tiles of queries at a time and KS of them per step
+  const int64_t all = int64_t((max_len + kRows - 1) / kRows) * group / p.kv_ks + 1;
+  const int64_t window =
+      std::min<int64_t>(all, ((int64_t(wl) + wr + kv_rows) / kRows + 1) * group / p.kv_ks + 1);
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(512 / (full * n_kv_heads * p.kv_ks),
+                                                        window / 6)));
+  p.sink_blocks = window < all ? std::min((ns + kv_rows - 1) / kv_rows, p.kv_blocks) : 0;
   const int64_t piece = std::max<int64_t>(6, window / p.splits);
   // (many sequences fill the GPU by themselves, and need no more than 256 MB of sums)
   const int64_t most = std::max<int64_t>(
@@ -785,77 +845,71 @@ BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t t
   const int64_t row = 2 * kHeadDim;
   p.kv_part = p.splits > 1 ? int64_t(p.splits) * n_kv_heads * total * row : 0;
   p.sink_part = p.sink_splits > 1 ? int64_t(n_seqs) * p.sink_splits * n_kv_heads *
-                                        p.sink_blocks * kBQ * row
+                                        p.sink_blocks * kv_rows * row
                                   : 0;
   p.bias_part = far > 0 ? int64_t(p.q_blocks) * n_seqs * n_heads * (2 * far + 1) : 0;
   p.norms = int64_t(p.q_blocks) * n_seqs * n_heads;
   return p;
 }
 
-hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* rel,
-                            hipStream_t st) {
-  const int nx = a.q_blocks;
-  const bool table = a.bias != nullptr, grad = dbias != nullptr;
+hipError_t launch_local_bwd(const LocalArgs& a, bool wide, bool norms, hipStream_t st) {
+  const bool table = a.bias != nullptr, grad = a.dbias != nullptr;
   const size_t tab = table ? size_t(bias_entries(a.far)) * 4 : 0;
-  const size_t lds_q = size_t(kStages) * kStageQ + tab * (grad ? 1 + kGradTables : 1) +
-                       (grad ? size_t(4) * kDiagFloats * 4 + 8 : 0);
-  const size_t lds_kv = size_t(kStages) * kStageKV + tab;
-  auto launch = [&](auto kernel, int x, int heads, size_t lds) {
-    // a large max distance needs more than the default limit of 64 KB
-    if (lds > 65536 - 2048) {
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               int(lds));
-      if (e != hipSuccess) return e;
-    }
-    hipLaunchKernelGGL(kernel, dim3(unsigned(grid_blocks(x, heads, a.n_seqs))), dim3(256), lds, st,
-                       a);
-    return hipGetLastError();
-  };
+  const size_t extra_q =
+      tab * (grad ? 1 + kGradTables : 1) + (grad ? size_t(4) * kDiagFloats * 4 + 8 : 0);
   const int hkv = a.n_heads / a.group;
-  auto run = [&](auto pos, auto drop, auto w) {
-    constexpr int P = decltype(pos)::value;
-    constexpr bool D = decltype(drop)::value, W = decltype(w)::value;
-    hipError_t e;
-    if constexpr (P == kPosTable)
-      e = grad ? launch(dq_kernel<P, D, true, W>, nx, a.n_heads, lds_q)
-               : launch(dq_kernel<P, D, false, W>, nx, a.n_heads, lds_q);
-    else
-      e = launch(dq_kernel<P, D, false, W>, nx, a.n_heads, lds_q);
-    if (e != hipSuccess) return e;
-    return launch(dkv_kernel<P, D, W>, kv_blocks(a), hkv, lds_kv);
-  };
-  using T_ = std::true_type;
-  using F_ = std::false_type;
-  auto pick = [&](auto pos) {
-    if (a.drop.on) return wide ? run(pos, T_{}, T_{}) : run(pos, T_{}, F_{});
-    return wide ? run(pos, F_{}, T_{}) : run(pos, F_{}, F_{});
-  };
-  if (a.kmax != nullptr) {
+  if (norms) {
     const hipError_t e = launch_key_norm_max(a.k, a.k_tok, a.k_head, a.total, hkv,
                                              const_cast<float*>(a.kmax), st);
     if (e != hipSuccess) return e;
   }
+  auto launch = [&](auto kernel, int64_t blocks, size_t lds) {
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), lds, st, a);
+    return hipGetLastError();
+  };
+  auto launch_q = [&](auto kernel, int ks) {
+    return launch(kernel, grid_blocks(a.q_blocks, a.n_heads, a.n_seqs),
+                  size_t(ks == 2 ? 4 : 3) * kPairQ + extra_q);
+  };
+  auto launch_kv = [&](auto kernel, int ks) {
+    return launch(kernel, grid_blocks(kv_blocks(a), hkv, a.n_seqs) + (grad ? a.n_heads : 0),
+                  size_t(ks == 2 ? 4 : 3) * kPairKV + tab);
+  };
+  auto run = [&](auto pos, auto drop) {
+    constexpr int P = decltype(pos)::value;
+    constexpr bool D = decltype(drop)::value;
+    constexpr bool G = P == kPosTable;  // (a bias gradient only where there is a table)
+    auto at = [&](auto w) {
+      constexpr bool W = decltype(w)::value;
+      hipError_t e;
+      if (a.ks == 2)
+        e = launch_q(dq_kernel<P, D, false, W, 2>, 2);
+      else
+        e = grad ? launch_q(dq_kernel<P, D, G, W, 1>, 1)
+                 : launch_q(dq_kernel<P, D, false, W, 1>, 1);
+      if (e != hipSuccess) return e;
+      return a.kv_ks == 2 ? launch_kv(dkv_kernel<P, D, W, 2>, 2)
+                          : launch_kv(dkv_kernel<P, D, W, 1>, 1);
+    };
+    return wide ? at(std::true_type{}) : at(std::false_type{});
+  };
+  auto pick = [&](auto pos) {
+    return a.drop.on ? run(pos, std::true_type{}) : run(pos, std::false_type{});
+  };
   hipError_t e = table ? pick(std::integral_constant<int, kPosTable>{})
                  : a.slopes != nullptr ? pick(std::integral_constant<int, kPosAlibi>{})
                                        : pick(std::integral_constant<int, kPosNone>{});
   if (e != hipSuccess) return e;
   if (a.splits > 1 || (a.sink_blocks > 0 && a.sink_splits > 1)) {
-    const int rows = a.splits > 1 ? nx : a.sink_blocks;
-    hipLaunchKernelGGL(kv_join_kernel, dim3(unsigned(rows * (kBQ / 32)), unsigned(hkv), unsigned(a.n_seqs)),
+    const int rows = (a.splits > 1 ? a.kv_blocks : a.sink_blocks) * (128 / a.kv_ks);
+    hipLaunchKernelGGL(kv_join_kernel,
+                       dim3(unsigned((rows + 31) / 32), unsigned(hkv), unsigned(a.n_seqs)),
                        dim3(256), 0, st, a);
     e = hipGetLastError();
-    if (e != hipSuccess) return e;
   }
-  if (!grad) return e;
-  const int E = 2 * a.far + 1;
-  hipLaunchKernelGGL(bias_sum_kernel, dim3(unsigned((E + 63) / 64), unsigned(a.n_heads)),
-                     dim3(1024), 0, st, a, E, rel);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(bias_bucket_kernel, dim3(unsigned(a.n_heads)), dim3(1024), size_t(E) * 8,
-                     st, a, E, rel, dbias);
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace attn

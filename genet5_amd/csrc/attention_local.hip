@@ -27,29 +27,33 @@ namespace g5moe {
 namespace attn {
 namespace {
 
-constexpr int kBQ = 128;
-constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kPairBytes = 2 * kTileBytes;  // a K tile, then its V tile
 
-template <int POS, bool DROP, bool WIDE>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(3, 3)))
+template <int POS, bool DROP, bool WIDE, int KS>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
 void local_fwd_kernel(LocalArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  using S = Split<KS>;
+  constexpr int kStageBytes = KS * kPairBytes;
   char* const ring = smem;
-  float* const tab = reinterpret_cast<float*>(smem + kStages * kStageBytes);
+  float* const tab = reinterpret_cast<float*>(smem + S::kStages * kStageBytes);
 
   int bx, hq, z;
-  if (!block_of(a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  if (!block_of(blockIdx.x, a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  if (POS == kPosAlibi && a.kmax != nullptr && a.n_heads <= 64)
+    by_slope(a.slopes, a.n_heads, a.n_seqs, hq, z);
   if (z == a.n_seqs - 1) zero_tail(a, a.o, a.o_tok, hq * a.o_head, bx, a.q_blocks);
   int s0, L;
   sequence(a, z, s0, L);
-  const int q0 = bx * kBQ;
+  const int q0 = bx * S::kOwn;
   if (q0 >= L) return;
   const int hk = hq / a.group;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int wq = q0 + wave * kCols;               // the wave's queries: wq .. wq_hi
+  const int tg = S::tile(wave);
+  const int wq = q0 + S::own(wave) * kCols;       // the wave's queries: wq .. wq_hi
   const int wq_hi = min(wq + kCols, L) - 1;
   const int iq = wq + col;
   const int wl = min(a.wl, L), wr = min(a.wr, L), ns = min(a.ns, L);
@@ -58,8 +62,49 @@ void local_fwd_kernel(LocalArgs a) {
   const float sl = POS == kPosAlibi ? a.slopes[hq] * kLog2e : 0.0f;
 
   bf16x8 qf[4];
-  load_own(qf, a.q + int64_t(s0 + min(iq, L - 1)) * a.q_tok + hq * a.q_head, half, iq < L,
-           a.sc < 0.0f ? 0x80008000u : 0u);
+  OwnRows qr;
+  qr.request(a.q + int64_t(s0 + min(iq, L - 1)) * a.q_tok + hq * a.q_head, half);
+
+  KeyTiles kt;
+  TilePair<WIDE> tiles;
+  tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
+  FragReader fr;
+  fr.init(lane);
+  const char* const kbase =
+      reinterpret_cast<const char*>(a.k + int64_t(s0) * a.k_tok + hk * a.k_head);
+  const char* const vbase =
+      reinterpret_cast<const char*>(a.v + int64_t(s0) * a.v_tok + hk * a.v_head);
+  // The next tile to load; past the last one it goes out again, into a buffer that no later
+  // tile reads, so that every step issues the same number of loads.
+  int n_is = 0;
+  auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < KS; ++g) {
+      tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff + g * kPairBytes);
+      n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
+    }
+  };
+  auto begin = [&](int reach) __attribute__((always_inline)) {
+    kt.init(q0, min(q0 + S::kOwn, L) - 1, L, min(wl, reach), min(wr, reach),
+            q0 - (ns - 1) > reach ? 0 : ns);
+    n_is = kt.first();
+#pragma unroll
+    for (int st = 0; st < S::kStages; ++st) issue(uint32_t(st) * kStageBytes);
+  };
+  if constexpr (POS != kPosAlibi) begin(L);
+  qr.take(qf, iq < L, a.sc < 0.0f ? 0x80008000u : 0u);
+  if constexpr (POS == kPosAlibi) {
+    // With the key norms, keys farther than `reach` from every query of the workgroup are left
+    // out: their probabilities are below 2^-64 of the query's own term, which it sees.
+    int reach = L;
+    if (a.kmax != nullptr) {
+      __shared__ float red[2][4];
+      float v[1] = {norm_max(qf)};
+      block_max(v, red, wave, lane);
+      reach = alibi_reach(2.0f * sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane), sl, L);
+    }
+    begin(reach);
+  }
   if constexpr (POS == kPosTable) {
     stage_bias(a, hq, tab);
     __syncthreads();
@@ -76,34 +121,6 @@ void local_fwd_kernel(LocalArgs a) {
     thr = min(a.drop.thr, 65535u) << 16;  // p = 1: the scale is 0
   }
 
-  // With ALiBi and the key norms, keys farther than `reach` from every query of the workgroup
-  // are left out: their probabilities are below 2^-64 of the query's own term, which it sees.
-  int reach = L;
-  if (POS == kPosAlibi && a.kmax != nullptr) {
-    __shared__ float red[2][4];
-    float v[1] = {norm_max(qf)};
-    block_max(v, red, wave, lane);
-    reach = alibi_reach(2.0f * sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane), sl, L);
-  }
-  KeyTiles kt;
-  kt.init(q0, min(q0 + kBQ, L) - 1, L, min(wl, reach), min(wr, reach),
-          q0 - (ns - 1) > reach ? 0 : ns);
-  TilePair<WIDE> tiles;
-  tiles.init(ring, wave, lane, L, a.k_tok * 2, a.v_tok * 2);
-  FragReader fr;
-  fr.init(lane);
-  const char* const kbase =
-      reinterpret_cast<const char*>(a.k + int64_t(s0) * a.k_tok + hk * a.k_head);
-  const char* const vbase =
-      reinterpret_cast<const char*>(a.v + int64_t(s0) * a.v_tok + hk * a.v_head);
-
-  // The next tile to load; past the last one it goes out again, into a buffer that no later
-  // tile reads, so that every step issues the same number of loads.
-  int n_is = kt.first();
-  auto issue = [&](uint32_t boff) __attribute__((always_inline)) {
-    tiles.issue(kbase, vbase, __builtin_amdgcn_readfirstlane(n_is), boff);
-    n_is = n_is < kt.w_hi ? kt.next(n_is) : n_is;
-  };
   f32x16 o[2] = {f32x16{}, f32x16{}};
   float m = -kInf, psum = 0.0f;
   float ms = 0.0f;  // what the exponents subtract: m, or 0 while every term was -inf
@@ -199,20 +216,19 @@ void local_fwd_kernel(LocalArgs a) {
       }
   };
 
-  int count = kt.s_end + kt.w_hi - kt.w_lo + 1;
   int n = kt.first();
+  if (tg == 1) n = kt.next(n);
   uint32_t boff = 0;
-#pragma unroll
-  for (int st = 0; st < kStages; ++st) issue(uint32_t(st) * kStageBytes);
-  gemm::wait_vmcnt<(kStages - 1) * 4>();
+  gemm::wait_vmcnt<(S::kStages - 1) * 4 * KS>();
   __syncthreads();
-  for (; count > 0; --count, n = kt.next(n)) {
+  for (int left = kt.count(); left > 0; left -= KS) {
     const int j0 = n * kRows, j1 = j0 + kRows - 1;
     // what the wave's queries see of the tile
-    const bool some = wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
+    const bool some =
+        left > tg && wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
     if (some) {
       const f32x16 zero16 = {};
-      const char* const K = ring + boff;
+      const char* const K = ring + boff + tg * kPairBytes;
       const char* const V = K + kTileBytes;
 #pragma unroll
       for (int kc = 0; kc < 4; ++kc)
@@ -248,16 +264,42 @@ void local_fwd_kernel(LocalArgs a) {
       }
     }
     // the next stage landed, and every wave has read all of this one
-    gemm::wait_vmcnt<(kStages - 2) * 4>();
+    gemm::wait_vmcnt<(S::kStages - 2) * 4 * KS>();
     __syncthreads();
     issue(boff);
-    boff = boff + kStageBytes == kStages * kStageBytes ? 0 : boff + kStageBytes;
+    boff = boff + kStageBytes == S::kStages * kStageBytes ? 0 : boff + kStageBytes;
+#pragma unroll
+    for (int g = 0; g < KS; ++g) n = kt.next(n);
   }
   // refills past the last tile may still be landing in this workgroup's LDS
   gemm::wait_vmcnt<0>();
 
+  float l = psum + __shfl_xor(psum, 32, 64);
+  if constexpr (KS == 2) {
+    // both waves' sums at the larger of their maxima
+    float* const other = reinterpret_cast<float*>(ring);
+    __syncthreads();
+    other[wave * 64 + lane] = m;
+    __syncthreads();
+    const float top = __builtin_fmaxf(m, other[(wave ^ 2) * 64 + lane]);
+    const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    float v[33];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      v[r] = o[0][r] * f;
+      v[16 + r] = o[1][r] * f;
+    }
+    v[32] = l * f;
+    if (!join_waves(v, ring + 1024, wave, lane)) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      o[0][r] = v[r];
+      o[1][r] = v[16 + r];
+    }
+    l = v[32];
+  }
   if (iq < L) {
-    const float l = psum + __shfl_xor(psum, 32, 64);
     const float inv = l == 0.0f ? 0.0f : (DROP ? a.drop.scale : 1.0f) / l;
     uint16_t* op = a.o + int64_t(s0 + iq) * a.o_tok + hq * a.o_head + 4 * half;
 #pragma unroll
@@ -280,6 +322,15 @@ __global__ __launch_bounds__(256) void zero_behind_kernel(LocalArgs a) {
 
 }  // namespace
 
+// Of 128-row blocks; a CU holds two workgroups.
+int pick_ks(int64_t blocks128) { return blocks128 < 256 ? 2 : 1; }
+
+// Dynamic LDS beyond the default limit of 64 KB (with room for the static).
+hipError_t allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 65536 - 2048) return hipSuccess;
+  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+}
+
 hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(zero_behind_kernel, dim3(16, unsigned(a.n_heads)), dim3(256), 0, st, a);
   return hipGetLastError();
@@ -292,23 +343,29 @@ hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st) {
                                              a.n_heads / a.group, const_cast<float*>(a.kmax), st);
     if (e != hipSuccess) return e;
   }
-  const size_t lds =
-      size_t(kStages) * kStageBytes + (a.bias != nullptr ? bias_entries(a.far) * 4 : 0);
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a); };
-  auto pick = [&](auto pos) {
-    constexpr int P = decltype(pos)::value;
-    if (a.drop.on)
-      wide ? launch(local_fwd_kernel<P, true, true>) : launch(local_fwd_kernel<P, true, false>);
-    else
-      wide ? launch(local_fwd_kernel<P, false, true>) : launch(local_fwd_kernel<P, false, false>);
+  auto launch = [&](auto kernel, int stages, int ks) {
+    const size_t lds = size_t(stages * ks) * kPairBytes +
+                       (a.bias != nullptr ? bias_entries(a.far) * 4 : 0);
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a);
+    return hipGetLastError();
   };
-  if (a.bias != nullptr)
-    pick(std::integral_constant<int, kPosTable>{});
-  else if (a.slopes != nullptr)
-    pick(std::integral_constant<int, kPosAlibi>{});
-  else
-    pick(std::integral_constant<int, kPosNone>{});
-  return hipGetLastError();
+  auto pick = [&](auto pos, auto drop) {
+    constexpr int P = decltype(pos)::value;
+    constexpr bool D = decltype(drop)::value;
+    if (wide)
+      return a.ks == 2 ? launch(local_fwd_kernel<P, D, true, 2>, 2, 2)
+                       : launch(local_fwd_kernel<P, D, true, 1>, 3, 1);
+    return a.ks == 2 ? launch(local_fwd_kernel<P, D, false, 2>, 2, 2)
+                     : launch(local_fwd_kernel<P, D, false, 1>, 3, 1);
+  };
+  auto with_drop = [&](auto pos) {
+    return a.drop.on ? pick(pos, std::true_type{}) : pick(pos, std::false_type{});
+  };
+  if (a.bias != nullptr) return with_drop(std::integral_constant<int, kPosTable>{});
+  if (a.slopes != nullptr) return with_drop(std::integral_constant<int, kPosAlibi>{});
+  return with_drop(std::integral_constant<int, kPosNone>{});
 }
 
 }  // namespace attn

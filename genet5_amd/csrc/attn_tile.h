@@ -34,7 +34,6 @@ constexpr int kCols = 32;                        // the wave's own rows
 constexpr int kRows = 64;                        // rows of a streamed tile
 constexpr int kRowBytes = kHeadDim * 2;
 constexpr int kTileBytes = kRows * kRowBytes;    // 8 KB
-constexpr int kStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_inff();
@@ -76,6 +75,18 @@ __device__ __forceinline__ void lds_dma16_v(const char* addr, uint32_t lds) {
                : "memory", "m0");
 }
 #pragma clang diagnostic pop
+
+// How the four waves of a workgroup share its work: KS = 1: each has 32 own rows, all of them
+// every tile; KS = 2: two waves share 32 own rows and take every second tile each, and their
+// sums are joined at the end.  The second needs twice the loads per product, and halves the
+// smallest unit of work: for launches of few workgroups.
+template <int KS>
+struct Split {
+  static constexpr int kOwn = 4 / KS * kCols;             // own rows per workgroup
+  static constexpr int kStages = KS == 1 ? 3 : 2;         // of KS tile pairs each
+  static __device__ __forceinline__ int own(int wave) { return KS == 1 ? wave : wave & 1; }
+  static __device__ __forceinline__ int tile(int wave) { return KS == 1 ? 0 : wave >> 1; }
+};
 
 // The DMA of one 64-row tile of each of two matrices by four waves (tile a, then tile b
 // 8 KB behind): instruction i of a wave fills rows 8 (4i + wave) .. + 8, so four instructions
@@ -166,23 +177,26 @@ struct FragReader {
   }
 };
 
-// The wave's own rows as a B operand: row `row` of a bf16 matrix (head dims 16 kc + 8 half
-// .. + 8), zeros where !ok.  The loads have landed when this returns, so that no wait for
-// them falls into the tile loop.
-__device__ __forceinline__ void load_own(bf16x8 (&f)[4], const uint16_t* p, int half, bool ok,
-                                         uint32_t flip) {
+// The wave's own rows as a B operand (head dims 16 kc + 8 half .. + 8): requested, so that
+// other loads go out behind them, and taken later, when they have landed, so that no wait for
+// them falls into the tile loop.  Zeros where !ok (the request still has to be in bounds).
+struct OwnRows {
   u32x4 w[4];
+  __device__ __forceinline__ void request(const uint16_t* p, int half) {
 #pragma unroll
-  for (int kc = 0; kc < 4; ++kc)
-    w[kc] = ok ? *reinterpret_cast<const u32x4*>(p + 16 * kc + 8 * half) : u32x4{0, 0, 0, 0};
-#pragma unroll
-  for (int kc = 0; kc < 4; ++kc) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[kc][e] ^= flip;
-    asm volatile("" : "+v"(w[kc]));
-    f[kc] = __builtin_bit_cast(bf16x8, w[kc]);
+    for (int kc = 0; kc < 4; ++kc)
+      w[kc] = *reinterpret_cast<const u32x4*>(p + 16 * kc + 8 * half);
   }
-}
+  __device__ __forceinline__ void take(bf16x8 (&f)[4], bool ok, uint32_t flip) {
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[kc][e] = ok ? w[kc][e] ^ flip : 0u;
+      asm volatile("" : "+v"(w[kc]));
+      f[kc] = __builtin_bit_cast(bf16x8, w[kc]);
+    }
+  }
+};
 
 // A 32-row block's accumulator elements packed to bf16: rows 16c .. + 16 as a B operand.
 __device__ __forceinline__ bf16x8 chunk(const uint32_t (&pk)[8], int c) {
@@ -256,16 +270,19 @@ struct LocalArgs {
   float* nl;                        // backward: -lse * log2(e), [n_heads, total]
   float* delta;                     // backward: dout . o, [n_heads, total]
   uint32_t* rowkey;                 // backward with dropout: the rows' keys, [n_heads, total]
-  float* part;                      // backward: bias sums per workgroup
+  float* part;                      // backward: bias sums per workgroup of dq_kernel
+  void* dbias;                      // backward: [n_buckets, n_heads] or nullptr
   int wl, wr, ns;                   // window (large = unlimited), first tokens always visible
   // with ALiBi, for leaving out tiles whose probabilities vanish, or nullptr: the largest key
   // norm of each 64-token block [n_kv_heads, ceil(total / 64)], and (backward) the largest
-  // query norm of each 128-query block [n_heads, n_seqs, q_blocks]
+  // query norm of each block of q_rows queries [n_heads, n_seqs, q_blocks]
   const float* kmax;
   float* qmax;
-  int q_blocks;
+  int q_blocks;                     // workgroups per head and sequence, of q_rows queries
+  int q_rows;
+  int ks, kv_ks;                    // Split of the kernels over queries and over keys
   // backward: the splits of a key block's query tiles (of the sinks' blocks) and their sums
-  int splits, sink_blocks, sink_splits;
+  int kv_blocks, splits, sink_blocks, sink_splits;
   float *kv_part, *sink_part;
   int64_t total;
   int max_len;                      // sequences are not computed past it
@@ -273,13 +290,13 @@ struct LocalArgs {
 };
 
 // The workgroup's (x, head, sequence) of nx x heads x sequences, from a one-dimensional grid of
-// grid_blocks() workgroups: consecutive workgroups go to the eight XCDs in turn, so runs of
+// grid_blocks() workgroups, id the number of this one: consecutive workgroups go to the eight XCDs in turn, so runs of
 // kRun blocks x of one head are given to one XCD, whose L2 then serves their common tiles.
 // False: nothing to do.
 constexpr int kXcds = 8;
 constexpr int kRun = 8;
-__device__ __forceinline__ bool block_of(int nx, int heads, int n_seqs, int& x, int& h, int& z) {
-  const uint32_t id = blockIdx.x;
+__device__ __forceinline__ bool block_of(uint32_t id, int nx, int heads, int n_seqs, int& x,
+                                         int& h, int& z) {
   const uint32_t j = id / kXcds;
   const uint32_t item = ((j / kRun) * kXcds + id % kXcds) * kRun + j % kRun;
   const uint32_t pair = item / uint32_t(nx);
@@ -287,6 +304,23 @@ __device__ __forceinline__ bool block_of(int nx, int heads, int n_seqs, int& x, 
   h = int(pair % uint32_t(heads));
   z = int(pair / uint32_t(heads));
   return z < n_seqs;
+}
+// The same in the order of falling work under ALiBi: heads by rising slope (the reach falls
+// with it), every sequence of a head before the next one's, so that the launch does not end
+// on its longest workgroups.  Up to 64 heads.
+__device__ __forceinline__ void by_slope(const float* slopes, int heads, int n_seqs, int& h,
+                                         int& z) {
+  const int pair = z * heads + h;
+  const int lane = threadIdx.x & 63;
+  const float own = lane < heads ? slopes[lane] : kInf;
+  const float key = own > 0.0f ? own : 0.0f;  // no reach
+  int rank = 0;
+  for (int j = 0; j < heads; ++j) {
+    const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(key), j));
+    rank += other < key || (other == key && j < lane) ? 1 : 0;
+  }
+  z = pair % n_seqs;
+  h = __builtin_ctzll(__ballot(lane < heads && rank == pair / n_seqs));
 }
 inline int64_t grid_blocks(int64_t nx, int64_t heads, int64_t n_seqs) {
   constexpr int64_t unit = kXcds * kRun;
@@ -299,6 +333,23 @@ __device__ __forceinline__ void sequence(const LocalArgs& a, int z, int& s0, int
   const int total = int(a.total);
   s0 = __builtin_amdgcn_readfirstlane(min(max(a.cu[z], 0), total));
   L = __builtin_amdgcn_readfirstlane(min(min(max(a.cu[z + 1], s0), total) - s0, a.max_len));
+}
+
+// KS = 2: the accumulators of waves 2 and 3 added to those of waves 0 and 1, by way of LDS
+// (N x 256 bytes per wave pair at buf).  Every wave calls it; true for those that hold the sum.
+template <int N>
+__device__ __forceinline__ bool join_waves(float (&v)[N], char* buf, int wave, int lane) {
+  float* const p = reinterpret_cast<float*>(buf) + (wave & 1) * N * 64 + lane;
+  __syncthreads();
+  if (wave >= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i * 64] = v[i];
+  }
+  __syncthreads();
+  if (wave >= 2) return false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += p[i * 64];
+  return true;
 }
 
 // Largest norm of the wave's own 32 rows (every lane).
@@ -387,6 +438,7 @@ struct KeyTiles {
   }
   __device__ __forceinline__ int first() const { return s_end > 0 ? 0 : w_lo; }
   __device__ __forceinline__ int next(int n) const { return n + 1 == s_end ? w_lo : n + 1; }
+  __device__ __forceinline__ int count() const { return s_end + w_hi - w_lo + 1; }
 };
 
 // The largest norm of each 64-token block of each head of k (attention.hip).
@@ -397,15 +449,18 @@ namespace attn {
 
 // Zeros in the rows of out behind the last sequence.
 hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st);
+// Split of a launch over blocks of 128 own rows.
+int pick_ks(int64_t blocks128);
+hipError_t allow_lds(const void* kernel, size_t bytes);
 // wide: a token stride of a streamed matrix of 2^24 elements or more.
 hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st);
-// dbias: [n_buckets, n_heads] out in the table's type, or nullptr; rel: [n_heads, 2 far + 1].
-hipError_t launch_local_bwd(const LocalArgs& a, bool wide, void* dbias, float* rel,
-                            hipStream_t st);
+// norms: a.kmax is to be written first.
+hipError_t launch_local_bwd(const LocalArgs& a, bool wide, bool norms, hipStream_t st);
 // The splits of the key/value gradients and the floats of the backward's buffers (far: the bias
 // table's largest distance, 0 without a table).
 struct BwdPlan {
-  int q_blocks, splits, sink_blocks, sink_splits;
+  int ks, q_blocks;                              // of dq_kernel
+  int kv_ks, kv_blocks, splits, sink_blocks, sink_splits;  // of dkv_kernel
   int64_t kv_part, sink_part, bias_part, norms;
 };
 BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t total, int wl,

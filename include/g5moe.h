@@ -674,7 +674,9 @@ g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
  * and softmax_lse and the same inputs, options and seed.
  *   dout : bf16, the gradient of out;  dq, dk, dv : bf16 out (the gradients of key and value
  *   heads summed over the query heads that share them);  dbias : [bias_buckets, n_heads] in
- *   bias_dtype out, or NULL;  ws : g5moe_attn_bwd_workspace_size() bytes, 256-byte aligned;
+ *   bias_dtype out, or NULL;  key_norms : the ws of the forward's call, which holds the key
+ *   norms where ALiBi uses them, or NULL (they are formed again);
+ *   ws : g5moe_attn_bwd_workspace_size() bytes, 256-byte aligned;
  *   grad_shape : shape with the strides of dq, dk, dv and (its o strides) dout.
  * Rows of dq, dk and dv behind the last sequence are set to 0.  Sums are fp32; P and dS enter
  * their products as bf16.  No atomics on memory; the order of every sum is fixed. */
@@ -682,9 +684,9 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
                             const void* out, const float* softmax_lse, const int32_t* cu_seqlens,
                             const float* alibi_slopes, const void* bias_table,
                             const int32_t* bucket_of, float softmax_scale, void* dq, void* dk,
-                            void* dv, void* dbias, void* ws, const g5moe_attn_options* options,
-                            const g5moe_attn_shape* shape, const g5moe_attn_shape* grad_shape,
-                            void* stream);
+                            void* dv, void* dbias, const float* key_norms, void* ws,
+                            const g5moe_attn_options* options, const g5moe_attn_shape* shape,
+                            const g5moe_attn_shape* grad_shape, void* stream);
 
 /* ---- Residual add with dropout ----------------------------------------------------
  * out = residual + alpha m x: `hidden_states + dropout(ff_output) * alpha`

@@ -191,7 +191,7 @@ def test_c_refusals(g5lib, opts, shape, ptrs, scale, match):
                   ctypes.byref(s), None)
     with pytest.raises(_lib.G5MoEError, match=match):
         _lib.call("g5moe_attn_bwd", FAKE, at["q"], at["k"], at["v"], at["out"], FAKE, at["cu"],
-                  at["slopes"], at["table"], at["lut"], scale, FAKE, FAKE, FAKE, None, FAKE,
+                  at["slopes"], at["table"], at["lut"], scale, FAKE, FAKE, FAKE, None, None, FAKE,
                   ctypes.byref(o), ctypes.byref(s), ctypes.byref(_shape(**shape)), None)
 
 
@@ -200,7 +200,7 @@ def test_c_backward_refusals(g5lib):
 
     def call(dbias=None, grad=s, ws=FAKE, lse=FAKE):
         _lib.call("g5moe_attn_bwd", FAKE, FAKE, FAKE, FAKE, FAKE, lse, FAKE, None, None, None,
-                  0.1, FAKE, FAKE, FAKE, dbias, ws, ctypes.byref(o), ctypes.byref(s),
+                  0.1, FAKE, FAKE, FAKE, dbias, None, ws, ctypes.byref(o), ctypes.byref(s),
                   ctypes.byref(grad), None)
 
     for kw, match in ((dict(dbias=FAKE), "dbias"), (dict(grad=_shape(total_tokens=9)), "strides"),
@@ -215,7 +215,8 @@ def test_c_empty_calls_do_nothing(g5lib):
         _lib.call("g5moe_attn_local_fwd", None, None, None, None, None, None, None, None, 0.1,
                   None, None, None, ctypes.byref(s), None)
         _lib.call("g5moe_attn_bwd", None, None, None, None, None, None, None, None, None, None,
-                  0.1, None, None, None, None, None, None, ctypes.byref(s), ctypes.byref(s), None)
+                  0.1, None, None, None, None, None, None, None, ctypes.byref(s), ctypes.byref(s),
+                  None)
 
 
 def test_workspace_size_counts_what_the_backward_keeps(g5lib):
@@ -234,15 +235,15 @@ def test_workspace_size_counts_what_the_backward_keeps(g5lib):
     assert size(_opts(), **kw) == base
     assert size(_opts(p=0.1), **kw) == base + up(8 * T)
     assert size(_opts(bias_buckets=8, bias_distance=10), **kw) == \
-        base + up(blocks * 16 * 8 * 21) + up(8 * 21)
+        base + up(blocks * 16 * 8 * 21)
     # sinks under a window: their 128 keys' tiles in pieces of the window's length
-    all_tiles, window = 40 * 2, ((100 + 128) // 64 + 1) * 2
-    pieces = -(-all_tiles // window)
+    all_steps, window = 40 * 2 + 1, ((100 + 128) // 64 + 1) * 2 + 1
+    pieces = -(-all_steps // window)
     assert size(_opts(window_left=50, window_right=50, sink_tokens=3), **kw) == \
         base + up(16 * pieces * 4 * 128 * 128)
-    # few tokens: every key block's tiles are split
+    # few tokens: blocks of 64 keys, and each one's tiles split over workgroups
     kw.update(total_tokens=1000, max_seqlen=1000, n_seqs=1)
-    assert size(_opts(), **kw) == 2 * up(8000) + up(4 * 16) + up(8 * 8) + up(5 * 4 * 1000 * 128)
+    assert size(_opts(), **kw) == 2 * up(8000) + up(4 * 16) + up(16 * 8) + up(2 * 4 * 1000 * 128)
 
 
 @pytest.mark.parametrize("args,match", [
