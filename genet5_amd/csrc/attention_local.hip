@@ -142,9 +142,10 @@ void local_fwd_kernel(LocalArgs a) {
         for (int r = 0; r < 16; ++r) o[mb][r] *= alpha;
     }
   };
-  // The softmax step of the scores in s (PLAIN: scores to be scaled, the tile's constant bias c
-  // to be added; else terms) and the output product, 32 keys at a time.
-  auto step = [&](auto plain_c, int n, float c, const char* V) __attribute__((always_inline)) {
+  // The softmax step: probabilities of the scores in s (PLAIN: scores to be scaled, the tile's
+  // constant bias c to be added; else terms).
+  uint32_t pk[2][8];
+  auto softmax = [&](auto plain_c, int n, float c) __attribute__((always_inline)) {
     constexpr bool PLAIN = decltype(plain_c)::value;
     float mx = s[0][0];
 #pragma unroll
@@ -160,8 +161,7 @@ void local_fwd_kernel(LocalArgs a) {
     const uint32_t jp = uint32_t(n * kRows + 4 * half) >> 1;
     float sum = 0.0f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      uint32_t pk[8];
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         float p[2];
@@ -177,17 +177,8 @@ void local_fwd_kernel(LocalArgs a) {
           p[0] = (bits << 16) >= thr ? p[0] : 0.0f;
           p[1] = bits >= thr ? p[1] : 0.0f;
         }
-        pk[r >> 1] = pack_bf16x2(p[0], p[1]);
+        pk[b][r >> 1] = pack_bf16x2(p[0], p[1]);
       }
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        const bf16x8 pf = chunk(pk, cc);
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
-          o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.trans(V, 2 * b + cc, mb), pf, o[mb],
-                                                          0, 0, 0);
-      }
-    }
     psum += sum;
   };
   // Per-element terms in place of the scores.
@@ -216,58 +207,117 @@ void local_fwd_kernel(LocalArgs a) {
       }
   };
 
-  int n = kt.first();
-  if (tg == 1) n = kt.next(n);
+  // Operands are read ahead: a tile's K fragments behind the previous tile's output product,
+  // its V fragments before the softmax.
   uint32_t boff = 0;
-  gemm::wait_vmcnt<(S::kStages - 1) * 4 * KS>();
-  __syncthreads();
-  for (int left = kt.count(); left > 0; left -= KS) {
-    const int j0 = n * kRows, j1 = j0 + kRows - 1;
-    // what the wave's queries see of the tile
-    const bool some =
-        left > tg && wq < L && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
-    if (some) {
-      const f32x16 zero16 = {};
-      const char* const K = ring + boff + tg * kPairBytes;
-      const char* const V = K + kTileBytes;
+  bf16x8 kf[2][4], vf[4][2];
+  auto load_kf = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int kc = 0; kc < 4; ++kc)
+    for (int kc = 0; kc < 4; ++kc)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(K, b, kc), qf[kc],
-                                                         kc == 0 ? zero16 : s[b], 0, 0, 0);
-      const bool all = j1 < L && ((j0 >= wq_hi - wl && j1 <= wq + wr) || j1 < ns);
-      using T_ = std::true_type;
-      using F_ = std::false_type;
-      float c = 0.0f;
-      bool look = false;
-      if constexpr (POS == kPosTable) {
-        const bool left = j1 - wq <= -a.far, right = j0 - wq_hi >= a.far;
-        look = !left && !right;
-        c = left ? far_l : far_r;
-      }
-      if constexpr (POS == kPosAlibi) {
-        const bool before = j1 <= wq, after = j0 >= wq_hi;
-        look = !(bc.ok && (before || after));
-        if (!look) bc.add(s, float(iq - j0), before);
-      }
-      if (all && !look) {
-        step(T_{}, n, c, V);
-      } else {
-        if (POS == kPosNone || !look)
-          terms(T_{}, F_{}, n, c);
-        else if (all)
-          terms(F_{}, T_{}, n, c);
-        else
-          terms(T_{}, T_{}, n, c);
-        step(F_{}, n, c, V);
-      }
-    }
+      for (int b = 0; b < 2; ++b) kf[b][kc] = fr.row(ring + boff + tg * kPairBytes, b, kc);
+  };
+  auto scores = [&]() __attribute__((always_inline)) {
+    const f32x16 zero16 = {};
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][kc], qf[kc],
+                                                       kc == 0 ? zero16 : s[b], 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+        vf[c][mb] = fr.trans(ring + boff + tg * kPairBytes + kTileBytes, c, mb);
+  };
+  auto turn = [&]() __attribute__((always_inline)) {
     // the next stage landed, and every wave has read all of this one
     gemm::wait_vmcnt<(S::kStages - 2) * 4 * KS>();
     __syncthreads();
     issue(boff);
     boff = boff + kStageBytes == S::kStages * kStageBytes ? 0 : boff + kStageBytes;
+    load_kf();
+  };
+  auto output = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bf16x8 pf = chunk(pk[c >> 1], c & 1);
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+        o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[c][mb], pf, o[mb], 0, 0, 0);
+    }
+  };
+  using T_ = std::true_type;
+  using F_ = std::false_type;
+
+  // The wave's plain tiles: [all_lo, all_hi] or up to sink_hi are wholly visible, and of those
+  // the ones up to before_hi or from after_lo have a bias of one kind.
+  const bool any = wq < L;
+  const int all_lo = any ? (max(wq_hi - wl, 0) + kRows - 1) / kRows : kNever;
+  const int all_hi = (min(wq + wr, L - 1) + 1) / kRows - 1;
+  const int sink_hi = any ? ns / kRows - 1 : -1;
+  int before_hi = -1, after_lo = 0;
+  if constexpr (POS == kPosTable) {
+    before_hi = ((wq - a.far + 1) >> 6) - 1;
+    after_lo = (wq_hi + a.far + kRows - 1) / kRows;
+  }
+  if constexpr (POS == kPosAlibi) {
+    before_hi = bc.ok ? (wq + 1) / kRows - 1 : -1;
+    after_lo = bc.ok ? (wq_hi + kRows - 1) / kRows : kNever;
+  }
+
+  int n = kt.first();
+  if (tg == 1) n = kt.next(n);
+  gemm::wait_vmcnt<(S::kStages - 1) * 4 * KS>();
+  __syncthreads();
+  load_kf();
+  for (int left = kt.count(); left > 0;) {
+    // a run of plain tiles of one kind, without branches
+    const bool before = POS != kPosNone && n <= before_hi;
+    int hi = n >= all_lo && n <= all_hi ? all_hi : n <= sink_hi ? sink_hi : -1;
+    if (POS != kPosNone) hi = before ? min(hi, before_hi) : n >= after_lo ? hi : -1;
+    if (n < kt.s_end) hi = min(hi, kt.s_end - 1);
+    const int run = min(hi >= n ? (hi - n) / KS + 1 : 0, (left - tg + KS - 1) / KS);
+    if (run > 0) {
+      const float c = before ? far_l : far_r;
+      float d = float(iq - n * kRows);
+      for (int i = 0; i < run; ++i) {
+        scores();
+        if constexpr (POS == kPosAlibi) {
+          bc.add(s, d, before);
+          d -= float(KS * kRows);
+        }
+        softmax(T_{}, n + i * KS, c);
+        turn();
+        output();
+      }
+      left -= run * KS;
+      n += (run - 1) * KS;
+    } else {
+      const int j0 = n * kRows, j1 = j0 + kRows - 1;
+      // what the wave's queries see of the tile
+      const bool some =
+          left > tg && any && ((j0 <= wq_hi + wr && j1 >= wq - wl) || j0 < ns);
+      if (some) {
+        scores();
+        const bool all = (n >= all_lo && n <= all_hi) || n <= sink_hi;
+        const bool look = POS != kPosNone && !before && !(n >= after_lo);
+        const float c = before ? far_l : far_r;
+        if constexpr (POS == kPosAlibi)
+          if (!look) bc.add(s, float(iq - j0), before);
+        if (!look)
+          terms(T_{}, F_{}, n, c);
+        else if (all)
+          terms(F_{}, T_{}, n, c);
+        else
+          terms(T_{}, T_{}, n, c);
+        softmax(F_{}, n, c);
+      }
+      turn();
+      if (some) output();
+      left -= KS;
+    }
 #pragma unroll
     for (int g = 0; g < KS; ++g) n = kt.next(n);
   }

@@ -37,6 +37,7 @@ constexpr int kTileBytes = kRows * kRowBytes;    // 8 KB
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_inff();
+constexpr int kNever = 0x7fffffff;
 // Entries of the bias table in LDS beyond the largest distance on either side: a tile that
 // reaches within that distance of the wave's rows holds distances up to 95 past it.
 constexpr int kBiasPad = 96;
