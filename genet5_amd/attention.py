@@ -332,9 +332,33 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     _check_cu(cu_seqlens, dev)
     _check_position(alibi_slopes, relative_bias, max_distance, H, dev)
     ops._require(softmax_lse, "softmax_lse", (H, T), torch.float32, dev)
+    if key_norms is not None and (
+            key_norms.device != dev or key_norms.dtype != torch.uint8
+            or key_norms.numel() < _lib.attn_workspace_size(T, H, Hkv, HEAD_DIM)):
+        raise ValueError("key_norms must be what attn_local_fwd returned for this call")
+    return _attn_bwd(dout, q, k, v, out, softmax_lse, cu_seqlens, alibi_slopes, relative_bias,
+                     key_norms, (int(max_seqlen), softmax_scale, max_distance, *window_size,
+                                 sink_tokens, dropout_p), dropout_seed, bias_grad)
+
+
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace_size(opts: tuple, dropout_p: float, sizes: tuple) -> int:
+    o = _lib.AttnOptions(*opts[:6], _lib.make_dropout(dropout_p, 0), 0)
+    s = _lib.AttnShape(*sizes)
+    n = ctypes.c_size_t(0)
+    _lib.call("g5moe_attn_bwd_workspace_size", ctypes.byref(o), ctypes.byref(s), ctypes.byref(n))
+    return int(n.value)
+
+
+def _attn_bwd(dout, q, k, v, out, softmax_lse, cu_seqlens, alibi_slopes, relative_bias, key_norms,
+              call, dropout_seed, bias_grad):
+    """attn_bwd on arguments that have been checked (saved by a forward)."""
+    max_seqlen, softmax_scale, max_distance, wl, wr, sink_tokens, dropout_p = call
+    dev = q.device
+    T, H, Hkv = q.shape[0], q.shape[1], k.shape[1]
     bias = None if relative_bias is None else relative_bias.contiguous()
     buckets = None if bias is None else _buckets_on(bias.shape[0], max_distance, dev)
-    n_seqs, max_seqlen = cu_seqlens.numel() - 1, int(max_seqlen)
+    n_seqs = cu_seqlens.numel() - 1
     empty = n_seqs == 0 or max_seqlen <= 0 or T == 0   # nothing is launched
     new = torch.zeros if empty else torch.empty
     dq, dk, dv = (new((T, h, HEAD_DIM), dtype=torch.bfloat16, device=dev) for h in (H, Hkv, Hkv))
@@ -344,15 +368,14 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     if empty:
         return dq, dk, dv, dbias
     sizes = (n_seqs, max_seqlen, T, H, Hkv, HEAD_DIM, 0)
-    shape = _lib.AttnShape(*sizes, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                           v.stride(0), v.stride(1), out.stride(0), out.stride(1))
-    gshape = _lib.AttnShape(*sizes, dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1),
-                            dv.stride(0), dv.stride(1), dout.stride(0), dout.stride(1))
-    opts = _options(*window_size, sink_tokens, dropout_p, dropout_seed, bias, max_distance)
-    n = ctypes.c_size_t(0)
-    _lib.call("g5moe_attn_bwd_workspace_size", ctypes.byref(opts), ctypes.byref(shape),
-              ctypes.byref(n))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    shape = _lib.AttnShape(*sizes, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                           *out.stride()[:2])
+    gshape = _lib.AttnShape(*sizes, *dq.stride()[:2], *dk.stride()[:2], *dv.stride()[:2],
+                            *dout.stride()[:2])
+    opts = _options(wl, wr, sink_tokens, dropout_p, dropout_seed, bias, max_distance)
+    ws = torch.empty(_bwd_workspace_size(
+        (wl, wr, sink_tokens, opts.bias_buckets, opts.bias_distance, opts.bias_dtype), dropout_p,
+        sizes), dtype=torch.uint8, device=dev)
     ops._call_on(dev, "g5moe_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                  _ptr(softmax_lse), _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias),
                  _ptr(buckets), ctypes.c_float(softmax_scale), _ptr(dq), _ptr(dk), _ptr(dv),
@@ -368,13 +391,11 @@ def _draw_seed() -> int:
 
 def _bwd_call(need_bias, dout, q, k, v, out, lse, cu, slopes, bias, norms, call, seed):
     """attn_bwd with dout brought into a form the kernel reads."""
-    max_seqlen, scale, max_distance, wl, wr, sinks, p = call
     st = dout.stride()
     if dout.dtype != torch.bfloat16 or st[2] != 1 or st[0] % 8 or st[1] % 8 \
             or dout.data_ptr() % 16:
         dout = dout.to(torch.bfloat16).contiguous()
-    return attn_bwd(dout, q, k, v, out, lse, cu, max_seqlen, scale, slopes, bias, max_distance,
-                    (wl, wr), sinks, p, seed, need_bias, norms)
+    return _attn_bwd(dout, q, k, v, out, lse, cu, slopes, bias, norms, call, seed, need_bias)
 
 
 class _AttnFunction(torch.autograd.Function):
@@ -597,7 +618,9 @@ def flash_attn_func(q, k, v, dropout_p=0.0, softmax_scale=None, causal=False,
 @dataclass
 class FlashAttentionConfig:
     """Fields of the reference's FlashAttentionConfig (lib/blocks/_flash_att.py:15-30)
-    plus `alibi` (slopes of Press et al. per head when True)."""
+    plus `alibi` (slopes of Press et al. per head when True), `sink_tokens` (first tokens that
+    stay visible outside window_size) and `num_buckets` (> 0: a learned position bias
+    [num_buckets, num_heads] over distances up to max_distance, in ALiBi's place)."""
     embed_dim: int = 768
     num_heads: int = 12
     num_kv_heads: int = None
@@ -605,8 +628,14 @@ class FlashAttentionConfig:
     dropout: float = 0.0
     window_size: tuple = (-1, -1)
     alibi: bool = True
+    sink_tokens: int = 0
+    num_buckets: int = 0
+    max_distance: int = 128
 
     def __post_init__(self):
+        if self.num_buckets:
+            _check_buckets(self.num_buckets, self.max_distance)
+            self.alibi = False
         if self.num_kv_heads is None:
             self.num_kv_heads = self.num_heads
         if self.head_dim is None:
@@ -617,7 +646,8 @@ class FlashAttention(nn.Module):
     """Bidirectional attention with optional varlen packing and ALiBi, mirroring
     the reference's FlashAttention (lib/blocks/_flash_att.py:38-98): bias-free
     q/k/v/o projections, GQA, softmax scale 1/sqrt(head_dim); forward returns
-    (out, None)."""
+    (out, None).  The config's window, sinks and learned bias apply in training and in
+    inference; in training mode its dropout applies to the probabilities and to the output."""
 
     def __init__(self, config: FlashAttentionConfig):
         super().__init__()
@@ -638,6 +668,9 @@ class FlashAttention(nn.Module):
         self.v = nn.Linear(config.embed_dim, self.kv_dim, bias=False)
         self.o = nn.Linear(config.num_heads * self.head_dim, config.embed_dim, bias=False)
         self.dropout = nn.Dropout(config.dropout)
+        # a row per bucket, a column per head; zeros: no bias until it is learned
+        self.relative_bias = nn.Parameter(
+            torch.zeros(config.num_buckets, config.num_heads)) if config.num_buckets else None
         # fp32 slopes kept outside the module's buffers, so that casting the model
         # to bf16 does not round them
         self._slopes = alibi_slopes(config.num_heads) if config.alibi else None
@@ -678,7 +711,8 @@ class FlashAttention(nn.Module):
             return False
         weights = [m.weight for m in proj]
         needs_grad = torch.is_grad_enabled() and (
-            hidden_states.requires_grad or any(w.requires_grad for w in weights))
+            hidden_states.requires_grad or any(w.requires_grad for w in weights)
+            or (self.relative_bias is not None and self.relative_bias.requires_grad))
         return (not needs_grad and hidden_states.is_cuda
                 and hidden_states.dtype == torch.bfloat16
                 and all(w.dtype == torch.bfloat16 for w in weights)
@@ -704,8 +738,11 @@ class FlashAttention(nn.Module):
             max_seqlen = L
         out = flash_attn_varlen_func(q, k, v, cu_seqlens, cu_seqlens, max_seqlen, max_seqlen,
                                      dropout_p=drop_p, softmax_scale=self.softmax_scale,
-                                     causal=False,
-                                     alibi_slopes=self.alibi_slopes(hidden_states.device))
+                                     causal=False, window_size=self.config.window_size,
+                                     alibi_slopes=self.alibi_slopes(hidden_states.device),
+                                     sink_tokens=self.config.sink_tokens,
+                                     relative_bias=self.relative_bias,
+                                     max_distance=self.config.max_distance)
         if fused:
             out = ops.linear(out.reshape(B * L, self.num_heads * self.head_dim),
                              self.o.weight).view(B, L, -1)

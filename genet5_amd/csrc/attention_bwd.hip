@@ -864,8 +864,6 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, bool norms, hipStream
     if (e != hipSuccess) return e;
   }
   auto launch = [&](auto kernel, int64_t blocks, size_t lds) {
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds);
-    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), lds, st, a);
     return hipGetLastError();
   };

@@ -375,12 +375,6 @@ __global__ __launch_bounds__(256) void zero_behind_kernel(LocalArgs a) {
 // Of 128-row blocks; a CU holds two workgroups.
 int pick_ks(int64_t blocks128) { return blocks128 < 256 ? 2 : 1; }
 
-// Dynamic LDS beyond the default limit of 64 KB (with room for the static).
-hipError_t allow_lds(const void* kernel, size_t bytes) {
-  if (bytes <= 65536 - 2048) return hipSuccess;
-  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-}
-
 hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(zero_behind_kernel, dim3(16, unsigned(a.n_heads)), dim3(256), 0, st, a);
   return hipGetLastError();
@@ -396,8 +390,6 @@ hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st) {
   auto launch = [&](auto kernel, int stages, int ks) {
     const size_t lds = size_t(stages * ks) * kPairBytes +
                        (a.bias != nullptr ? bias_entries(a.far) * 4 : 0);
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds);
-    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a);
     return hipGetLastError();
   };

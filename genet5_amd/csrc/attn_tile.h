@@ -452,7 +452,6 @@ namespace attn {
 hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st);
 // Split of a launch over blocks of 128 own rows.
 int pick_ks(int64_t blocks128);
-hipError_t allow_lds(const void* kernel, size_t bytes);
 // wide: a token stride of a streamed matrix of 2^24 elements or more.
 hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st);
 // norms: a.kmax is to be written first.

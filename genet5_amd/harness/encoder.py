@@ -40,23 +40,39 @@ import torch.nn.functional as F
 from .. import attention, ops
 from ..attention import alibi_slopes  # noqa: F401  (re-exported for the harness)
 from ..moe import MoEFeedForward
+from ..residual import dropout_add
 from .blocks import RMSNorm
 
 
 class ALiBiSelfAttention(nn.Module):
     """Bidirectional self-attention with symmetric ALiBi, bias-free q/k/v/o.
 
-    backend "hip" (default): the HIP kernel through genet5_amd.attention's
+    backend "hip" (default): the HIP kernels through genet5_amd.attention's
     flash_attn_varlen_func (the call GeneT5's FlashAttention makes,
-    lib/blocks/_flash_att.py:76-88), forward-only, head_dim 64.
-    backend "torch": the reference composition in PyTorch, SDPA with the ALiBi
-    bias as an explicit mask, one call per packed sequence."""
+    lib/blocks/_flash_att.py:76-88), head_dim 64, forward and backward.
+    backend "torch": the reference composition in PyTorch, SDPA with the
+    bias as an explicit mask, one call per packed sequence.
 
-    def __init__(self, embed_dim: int, num_heads: int, backend: str = "hip"):
+    window_size, sink_tokens: local attention as flash_attn_varlen_func takes it.
+    num_buckets > 0: a learned bias [num_buckets, num_heads] over bucketed relative
+    positions up to max_distance, in ALiBi's place.  dropout: of the probabilities, in
+    training mode (the HIP backend's counter-based mask, SDPA's own with "torch")."""
+
+    def __init__(self, embed_dim: int, num_heads: int, backend: str = "hip",
+                 window_size: tuple = (-1, -1), sink_tokens: int = 0, num_buckets: int = 0,
+                 max_distance: int = 128, dropout: float = 0.0):
         super().__init__()
         if backend not in ("hip", "torch"):
             raise ValueError(f"attention backend {backend!r} is neither 'hip' nor 'torch'")
         self.backend = backend
+        self.window_size = tuple(window_size)
+        self.sink_tokens = sink_tokens
+        self.max_distance = max_distance
+        self.dropout = dropout
+        self.relative_bias = None
+        if num_buckets:
+            attention._check_buckets(num_buckets, max_distance)
+            self.relative_bias = nn.Parameter(torch.zeros(num_buckets, num_heads))
         self.num_heads = num_heads
         self.head_dim = embed_dim // num_heads
         self.q = nn.Linear(embed_dim, embed_dim, bias=False)
@@ -91,12 +107,36 @@ class ALiBiSelfAttention(nn.Module):
             self._bias_cache = {key: b}  # keep only the latest length
         return b
 
+    def position_bias(self, L: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+        """[1, heads, L, L]: the bias added to the scaled scores, -inf where the window and the
+        sinks leave a key out."""
+        if self.relative_bias is None and self.window_size == (-1, -1):
+            return self.alibi_bias(L, dtype, device)
+        pos = torch.arange(L, device=device)
+        rel = pos[None, :] - pos[:, None]
+        if self.relative_bias is None:
+            bias = self.alibi_bias(L, dtype, device)
+        else:
+            far = self.max_distance
+            lut = attention.relative_buckets(self.relative_bias.shape[0], far, device).long()
+            bias = self.relative_bias.to(dtype)[lut[rel.clamp(-far, far) + far]]
+            bias = bias.permute(2, 0, 1).unsqueeze(0)
+        wl, wr = self.window_size
+        hidden = torch.zeros_like(rel, dtype=torch.bool)
+        if wl >= 0:
+            hidden |= rel < -wl
+        if wr >= 0:
+            hidden |= rel > wr
+        return bias.masked_fill(hidden & (pos[None, :] >= self.sink_tokens), float("-inf"))
+
     def _attend(self, h: torch.Tensor) -> torch.Tensor:
         B, L, D = h.shape
         q = self.q(h).view(B, L, self.num_heads, self.head_dim).transpose(1, 2)
         k = self.k(h).view(B, L, self.num_heads, self.head_dim).transpose(1, 2)
         v = self.v(h).view(B, L, self.num_heads, self.head_dim).transpose(1, 2)
-        out = F.scaled_dot_product_attention(q, k, v, attn_mask=self.alibi_bias(L, q.dtype, q.device),
+        out = F.scaled_dot_product_attention(q, k, v, attn_mask=self.position_bias(L, q.dtype,
+                                                                          q.device),
+                                             dropout_p=self.dropout if self.training else 0.0,
                                              scale=1.0 / math.sqrt(self.head_dim))
         return self.o(out.transpose(1, 2).reshape(B, L, D))
 
@@ -127,7 +167,11 @@ class ALiBiSelfAttention(nn.Module):
         B, L, D = h.shape
         H, hd = self.num_heads, self.head_dim
         # one projection for q, k and v; the kernel reads them as strided views
-        qkv = self.project(h.reshape(B * L, D), self.qkv_weight()).view(B * L, 3, H, hd)
+        needs_grad = torch.is_grad_enabled() and (
+            h.requires_grad or any(p.requires_grad for p in self.parameters()))
+        w = torch.cat([self.q.weight, self.k.weight, self.v.weight]) if needs_grad \
+            else self.qkv_weight()
+        qkv = self.project(h.reshape(B * L, D), w).view(B * L, 3, H, hd)
         q, k, v = qkv[:, 0], qkv[:, 1], qkv[:, 2]
         if cu_seqlens is None:
             key = (B, L, h.device)
@@ -141,8 +185,14 @@ class ALiBiSelfAttention(nn.Module):
             cu = torch.tensor(bounds, dtype=torch.int32, device=h.device)
             max_len = max((b - a for a, b in zip(bounds[:-1], bounds[1:])), default=0)
         out = attention.flash_attn_varlen_func(q, k, v, cu, cu, max_len, max_len,
+                                               self.dropout if self.training else 0.0,
                                                softmax_scale=1.0 / math.sqrt(hd),
-                                               alibi_slopes=self.slopes_on(h.device))
+                                               window_size=self.window_size,
+                                               alibi_slopes=None if self.relative_bias is not None
+                                               else self.slopes_on(h.device),
+                                               sink_tokens=self.sink_tokens,
+                                               relative_bias=self.relative_bias,
+                                               max_distance=self.max_distance)
         return self.project(out.view(B * L, D), self.o.weight).view(B, L, D)
 
     def forward(self, h: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -160,19 +210,30 @@ class MoEEncoderBlock(nn.Module):
     """fused (default): the attention output, the residual add, norm2, the router and
     the MoE's own residual add run as MoEFeedForward.residual_block (the
     fused_add_norm path of encoder.py:80-83).  fused = False: the non-fused path of
-    encoder.py:84-89 in torch around the MoE module."""
+    encoder.py:84-89 in torch around the MoE module.
+
+    dropout (training mode only): of the attention's probabilities, of the experts' hidden
+    state, and of both halves' outputs in the residual adds (genet5_amd.residual.dropout_add,
+    `hidden_states + dropout(ff_output) * alpha`, encoder.py:89).  attention_options: the
+    keyword arguments of ALiBiSelfAttention."""
 
     def __init__(self, embed_dim: int, num_heads: int, ff_dim: int, num_experts: int = 16,
-                 top_k: int = 2, attention_backend: str = "hip"):
+                 top_k: int = 2, attention_backend: str = "hip", dropout: float = 0.0,
+                 attention_options: Optional[dict] = None):
         super().__init__()
         self.norm1 = RMSNorm(embed_dim)
-        self.self_attn = ALiBiSelfAttention(embed_dim, num_heads, attention_backend)
+        self.self_attn = ALiBiSelfAttention(embed_dim, num_heads, attention_backend,
+                                            dropout=dropout, **(attention_options or {}))
         self.norm2 = RMSNorm(embed_dim)
-        self.ff = MoEFeedForward(embed_dim, ff_dim, 0.0, "silu", num_experts, top_k)
+        self.ff = MoEFeedForward(embed_dim, ff_dim, dropout, "silu", num_experts, top_k)
+        self.dropout = dropout
         self.fused = True
 
     def forward(self, h: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
         a = self.self_attn(self.norm1(h), cu_seqlens)
+        if self.training and self.dropout > 0:
+            h = dropout_add(a, h, self.dropout)
+            return dropout_add(self.ff(self.norm2(h)), h, self.dropout)
         if self.fused:
             return self.ff.residual_block(h, self.norm2.weight, self.norm2.variance_epsilon,
                                           x_add=a)
@@ -185,11 +246,13 @@ class GeneT5MoE(nn.Module):
 
     def __init__(self, vocab_size: int = 4096, embed_dim: int = 768, num_layers: int = 12,
                  num_heads: int = 12, ff_dim: int = 3072, num_experts: int = 16,
-                 top_k: int = 2, attention_backend: str = "hip"):
+                 top_k: int = 2, attention_backend: str = "hip", dropout: float = 0.0,
+                 attention_options: Optional[dict] = None):
         super().__init__()
         self.embed = nn.Embedding(vocab_size, embed_dim)
         self.layers = nn.ModuleList([
-            MoEEncoderBlock(embed_dim, num_heads, ff_dim, num_experts, top_k, attention_backend)
+            MoEEncoderBlock(embed_dim, num_heads, ff_dim, num_experts, top_k, attention_backend,
+                            dropout, attention_options)
             for _ in range(num_layers)])
         self.final_norm = RMSNorm(embed_dim)
         self.lm_head = nn.Linear(embed_dim, vocab_size, bias=False)

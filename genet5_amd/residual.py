@@ -125,11 +125,13 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor, p: float, alpha: float 
     if x.numel() == 0:
         return residual + x * alpha
     p, alpha = float(p) if training else 0.0, float(alpha)
-    x2, r2 = x.reshape(-1, d).contiguous(), residual.reshape(-1, d).contiguous()
+    x2, r2 = x, residual
+    if x.dim() != 2 or not (x.is_contiguous() and residual.is_contiguous()):
+        x2, r2 = x.reshape(-1, d).contiguous(), residual.reshape(-1, d).contiguous()
     if torch.compiler.is_compiling():
         out, _ = _dropout_add_op(x2, r2, p, alpha, None if seed is None else int(seed))
     else:
         if seed is None:
             seed = _draw_seed() if p > 0 else 0
         out = _DropoutAdd.apply(x2, r2, p, alpha, int(seed))
-    return out.view(x.shape)
+    return out if x2 is x else out.view(x.shape)
