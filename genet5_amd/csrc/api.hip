@@ -1105,7 +1105,7 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   a.sink_part = reinterpret_cast<float*>(base + w.sink_part);
   if (use_norms(a)) {
     a.kmax = key_norms != nullptr ? key_norms : reinterpret_cast<float*>(base + w.kmax);
-    a.qmax = reinterpret_cast<float*>(base + w.qmax);
+    a.qmax = reinterpret_cast<float2*>(base + w.qmax);
   }
   a.dbias = dbias;
   a.nl = reinterpret_cast<float*>(base + w.nl);

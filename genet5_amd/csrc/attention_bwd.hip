@@ -124,7 +124,7 @@ void dq_kernel(LocalArgs a) {
   asm volatile("" : "+v"(nl));
   if constexpr (POS == kPosAlibi) {
     // With the key norms, keys farther than `reach` from every query of the workgroup are left
-    // out: P_ij <= 2^(|q||k| sc - sl |i - j| - lse_i log2(e)) < 2^-64 there.
+    // out: P_ij <= 2^(|q||k| sc - sl |i - j| - lse_i log2(e)) < 2^-40 there.
     int reach = L;
     if (a.kmax != nullptr) {
       float v[2] = {norm_max(qf), nl};
@@ -132,7 +132,8 @@ void dq_kernel(LocalArgs a) {
       block_max(v, red, wave, lane);
       const float bound = __builtin_fabsf(sc) * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
       reach = alibi_reach(bound + v[1], sl, L);
-      if (tid == 0) a.qmax[(int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx] = v[0];
+      if (tid == 0)
+        a.qmax[(int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx] = float2{v[0], v[1]};
     }
     begin(reach);
   }
@@ -498,21 +499,22 @@ void dkv_kernel(LocalArgs a) {
   if constexpr (POS == kPosAlibi) kr.take(kf, own, 0u);
 
   // query tiles that see one of the workgroup's keys; with ALiBi and norms not those farther
-  // than `reach` from all of them (lse_i >= -|q||k| sc, the term of key i itself)
+  // than `reach` from all of them, by the same bound
   int reach = L;
   if (POS == kPosAlibi && a.qmax != nullptr) {
     __shared__ float red[2][4];
-    float v[1] = {norm_max(kf)};
-    block_max(v, red, wave, lane);
+    float kn[1] = {norm_max(kf)};
+    block_max(kn, red, wave, lane);
     reach = 0;
     for (int g = 0; g < a.group; ++g) {
       const int h = hk * a.group + g;
-      const float* p = a.qmax + (int64_t(h) * a.n_seqs + z) * a.q_blocks;
-      float qn[1] = {0.0f};
-      for (int i = tid; i < (L + a.q_rows - 1) / a.q_rows; i += 256) qn[0] = __builtin_fmaxf(qn[0], p[i]);
-      block_max(qn, red, wave, lane);
-      reach = max(reach, alibi_reach(2.0f * __builtin_fabsf(sc) * qn[0] * v[0],
-                                     a.slopes[h] * kLog2e, L));
+      const float2* p = a.qmax + (int64_t(h) * a.n_seqs + z) * a.q_blocks;
+      float top[1] = {-kInf};
+      for (int i = tid; i < (L + a.q_rows - 1) / a.q_rows; i += 256)
+        top[0] = __builtin_fmaxf(top[0],
+                                 __builtin_fmaf(__builtin_fabsf(sc) * kn[0], p[i].x, p[i].y));
+      block_max(top, red, wave, lane);
+      reach = max(reach, alibi_reach(top[0], a.slopes[h] * kLog2e, L));
     }
   }
   const int k_hi = min(k0 + S::kOwn, L) - 1;
@@ -865,7 +867,7 @@ BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t t
                                         p.sink_blocks * kv_rows * row
                                   : 0;
   p.bias_part = far > 0 ? int64_t(p.q_blocks) * n_seqs * n_heads * (2 * far + 1) : 0;
-  p.norms = int64_t(p.q_blocks) * n_seqs * n_heads;
+  p.norms = 2 * int64_t(p.q_blocks) * n_seqs * n_heads;
   return p;
 }
 

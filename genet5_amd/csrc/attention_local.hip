@@ -95,13 +95,25 @@ void local_fwd_kernel(LocalArgs a) {
   qr.take(qf, iq < L, a.sc < 0.0f ? 0x80008000u : 0u);
   if constexpr (POS == kPosAlibi) {
     // With the key norms, keys farther than `reach` from every query of the workgroup are left
-    // out: their probabilities are below 2^-64 of the query's own term, which it sees.
+    // out: their terms are below 2^-40 of the query's own key's, which it sees.
     int reach = L;
     if (a.kmax != nullptr) {
+      OwnRows kr;
+      kr.request(a.k + int64_t(s0 + min(iq, L - 1)) * a.k_tok + hk * a.k_head, half);
+      bf16x8 kf[4];
+      kr.take(kf, iq < L, 0u);
+      float dot = 0.0f;
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          dot = __builtin_fmaf(float(qf[kc][e]), float(kf[kc][e]), dot);
+      dot += __shfl_xor(dot, 32, 64);
       __shared__ float red[2][4];
-      float v[1] = {norm_max(qf)};
+      float v[2] = {norm_max(qf), iq < L ? -sc * dot : -kInf};
       block_max(v, red, wave, lane);
-      reach = alibi_reach(2.0f * sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane), sl, L);
+      const float bound = sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
+      reach = alibi_reach(bound + v[1], sl, L);
     }
     begin(reach);
   }

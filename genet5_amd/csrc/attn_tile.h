@@ -276,9 +276,10 @@ struct LocalArgs {
   int wl, wr, ns;                   // window (large = unlimited), first tokens always visible
   // with ALiBi, for leaving out tiles whose probabilities vanish, or nullptr: the largest key
   // norm of each 64-token block [n_kv_heads, ceil(total / 64)], and (backward) the largest
-  // query norm of each block of q_rows queries [n_heads, n_seqs, q_blocks]
+  // query norm and the largest -lse log2(e) of each block of q_rows queries
+  // [n_heads, n_seqs, q_blocks]
   const float* kmax;
-  float* qmax;
+  float2* qmax;
   int q_blocks;                     // workgroups per head and sequence, of q_rows queries
   int q_rows;
   int ks, kv_ks;                    // Split of the kernels over queries and over keys
@@ -394,9 +395,12 @@ __device__ __forceinline__ float key_norm(const LocalArgs& a, int hk, int s0, in
 }
 
 // The distance from which ALiBi's slope sl (times log2(e)) puts 2^(top - sl distance) below
-// 2^-64; L where there is none (also for an infinite or NaN top).
+// 2^-40; L where there is none (also for an infinite or NaN top).  The terms left out fall
+// geometrically from there: together they are below 2^-39 / (1 - 2^-sl), and a reach within a
+// sequence of length L means sl > 40 / L, so below L 2^-43: 2^-24, the rounding of one fp32
+// term, for a million tokens.
 __device__ __forceinline__ int alibi_reach(float top, float sl, int L) {
-  const float w = (top + 64.0f) / sl;
+  const float w = (top + 40.0f) / sl;
   return __builtin_amdgcn_readfirstlane(sl > 0.0f && w < float(L) ? max(int(w) + 1, 0) : L);
 }
 

@@ -231,7 +231,7 @@ def test_workspace_size_counts_what_the_backward_keeps(g5lib):
     up = lambda floats: (floats * 4 + 255) // 256 * 256
     T, blocks = 40000, 20
     kw = dict(total_tokens=T, max_seqlen=2500, n_seqs=16, n_heads=8, n_kv_heads=4)
-    base = 2 * up(8 * T) + up(4 * T // 64) + up(blocks * 16 * 8)
+    base = 2 * up(8 * T) + up(4 * T // 64) + up(2 * blocks * 16 * 8)
     assert size(_opts(), **kw) == base
     assert size(_opts(p=0.1), **kw) == base + up(8 * T)
     assert size(_opts(bias_buckets=8, bias_distance=10), **kw) == \
@@ -243,7 +243,7 @@ def test_workspace_size_counts_what_the_backward_keeps(g5lib):
         base + up(16 * pieces * 4 * 128 * 128)
     # few tokens: blocks of 64 keys, and each one's tiles split over workgroups
     kw.update(total_tokens=1000, max_seqlen=1000, n_seqs=1)
-    assert size(_opts(), **kw) == 2 * up(8000) + up(4 * 16) + up(16 * 8) + up(2 * 4 * 1000 * 128)
+    assert size(_opts(), **kw) == 2 * up(8000) + up(4 * 16) + up(2 * 16 * 8) + up(2 * 4 * 1000 * 128)
 
 
 @pytest.mark.parametrize("args,match", [
