@@ -294,7 +294,7 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     opts = _options(*window_size, sink_tokens, dropout_p, dropout_seed, bias, max_distance)
     ws = None
     if bias is None and (alibi_slopes is not None or dropout_p == 0):
-        # for the key norms: ALiBi's reach, the full attention's bounds
+        # for the key norms: ALiBi's reach, the bounds of long calls without any option
         ws = torch.empty(_lib.attn_workspace_size(T, H, Hkv, HEAD_DIM), dtype=torch.uint8,
                          device=dev)
     ops._call_on(dev, "g5moe_attn_local_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out),

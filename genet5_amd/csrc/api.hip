@@ -972,8 +972,13 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
   a.lse = softmax_lse;
   const bool full =
       options == nullptr || (options->window_left < 0 && options->window_right < 0);
-  if (full && bias_table == nullptr && !a.drop.on) {
-    // no option is in use: the full attention's kernel
+  if (full && bias_table == nullptr && !a.drop.on && alibi_slopes == nullptr &&
+      a.max_len > 2048) {
+    // Long sequences without any option: the full attention's kernel, whose loop with a fixed
+    // reference maximum is the faster one (12 heads, it against the kernel below: 8 x 4,550
+    // 606, 675 us; 2 x 4,550 171, 210; but 1 x 2,048 31, 29 and 4 x 1,100 31.5, 31; with ALiBi
+    // 8 x 4,550 357, 298; 2 x 4,550 109, 89; 4 x 1,100 31, 28, for the reach below is the
+    // tighter).
     g5moe_attn_shape f = s;
     f.max_seqlen = a.max_len;
     const hipError_t e = launch_attn_fwd(a.q, a.k, a.v, a.o, cu_seqlens, alibi_slopes,

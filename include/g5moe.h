@@ -652,8 +652,8 @@ typedef struct g5moe_attn_options {
  *   softmax_lse : fp32 [n_heads, total_tokens] out or NULL;  options : NULL = no window, no
  *   dropout;  ws : g5moe_attn_workspace_size() bytes or NULL, for the key norms with which
  *   keys whose probabilities vanish in fp32 under ALiBi are left out (each below 2^-40 of the
- *   row's largest), and which g5moe_attn_varlen_fwd (whose kernel computes a call without
- *   window, table and dropout) bounds its terms with.
+ *   row's largest), and which g5moe_attn_varlen_fwd (whose kernel computes long calls
+ *   without any option) bounds its terms with.
  * Rows of out behind the last sequence are set to 0 (of softmax_lse, left as they were).
  * Scores, softmax and sums are fp32, the probabilities enter the output product as bf16. */
 g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
