@@ -927,9 +927,10 @@ static g5moe_status local_args(attn::LocalArgs* a, const int32_t* cu_seqlens,
   a->total = s.total_tokens;
   a->max_len = int(std::min<int64_t>(s.max_seqlen, s.total_tokens));
   // a launch has less than 2^32 work-items, 256 per block
-  if (int64_t((a->max_len + 127) / 128) * s.n_heads * s.n_seqs > (int64_t(1) << 23))
-    return fail(G5MOE_ERR_UNSUPPORTED, "%d sequences of up to %d tokens and %d heads make more "
-                "than 2^23 blocks of 128 queries", int(s.n_seqs), a->max_len, int(s.n_heads));
+  if ((s.total_tokens / 128 + s.n_seqs) * s.n_heads > (int64_t(1) << 23))
+    return fail(G5MOE_ERR_UNSUPPORTED, "%lld tokens in %d sequences and %d heads make more than "
+                "2^23 blocks of 128 queries", (long long)s.total_tokens, int(s.n_seqs),
+                int(s.n_heads));
   a->q_tok = s.q_token_stride;
   a->k_tok = s.k_token_stride;
   a->v_tok = s.v_token_stride;
@@ -989,9 +990,9 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
   }
   if (use_norms(a)) a.kmax = static_cast<float*>(ws);
   const bool wide = std::max(s.k_token_stride, s.v_token_stride) >= (int64_t(1) << 24);
-  a.ks = attn::pick_ks((s.total_tokens / 128 + s.n_seqs) * s.n_heads);
-  a.q_rows = 128 / a.ks;
-  a.q_blocks = (a.max_len + a.q_rows - 1) / a.q_rows;
+  a.qb.init(a.total, a.n_seqs, a.max_len, 7);
+  a.ks = attn::pick_ks(int64_t(a.qb.count) * a.n_heads);
+  if (a.ks == 2) a.qb.init(a.total, a.n_seqs, a.max_len, 6);
   return hip_status(attn::launch_local_fwd(a, wide, as_stream(stream)),
                     "g5moe_attn_local_fwd");
 }
@@ -1099,10 +1100,9 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   const AttnBwdLayout w = attn_bwd_layout(a, plan);
   char* const base = static_cast<char*>(ws);
   a.ks = plan.ks;
-  a.q_rows = 128 / plan.ks;
-  a.q_blocks = plan.q_blocks;
+  a.qb = plan.qb;
   a.kv_ks = plan.kv_ks;
-  a.kv_blocks = plan.kv_blocks;
+  a.kb = plan.kb;
   a.splits = plan.splits;
   a.sink_blocks = plan.sink_blocks;
   a.sink_splits = plan.sink_splits;

@@ -51,18 +51,16 @@ void dq_kernel(LocalArgs a) {
   float* const gtab = tab + n_tab;
   float* const diag = gtab + (DBIAS ? kGradTables * n_tab + (n_tab & 1) : 0);  // 8-byte aligned
 
-  int bx, hq, z;
-  if (!block_of(blockIdx.x, a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  int slot, hq;
+  if (!block_of(blockIdx.x, a.qb.count, a.n_heads, slot, hq)) return;
   if (POS == kPosAlibi && a.kmax != nullptr && a.n_heads <= 64)
-    by_slope(a.slopes, a.n_heads, a.n_seqs, hq, z);
-  if (z == a.n_seqs - 1) zero_tail(a, a.dq, a.dq_tok, hq * a.dq_head, bx, a.q_blocks);
-  int s0, L;
-  sequence(a, z, s0, L);
-  const int q0 = bx * S::kOwn;
-  if (q0 >= L) {
+    hq = by_slope(a.slopes, a.n_heads, hq);
+  zero_tail(a, a.dq, a.dq_tok, hq * a.dq_head, slot, a.qb.count);
+  int z, s0, L, q0;
+  if (!find_block(a, a.qb, slot, z, s0, L, q0)) {
     if constexpr (DBIAS) {  // the sums by distance of no query
       const int E = 2 * a.far + 1;
-      float* out = a.part + ((int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx) * E;
+      float* out = a.part + (int64_t(hq) * a.qb.count + slot) * E;
       for (int x = threadIdx.x; x < E; x += 256) out[x] = 0.0f;
     }
     return;
@@ -133,7 +131,7 @@ void dq_kernel(LocalArgs a) {
       const float bound = __builtin_fabsf(sc) * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
       reach = alibi_reach(bound + v[1], sl, L);
       if (tid == 0)
-        a.qmax[(int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx] = float2{v[0], v[1]};
+        a.qmax[int64_t(hq) * a.qb.count + slot] = float2{v[0], v[1]};
     }
     begin(reach);
   }
@@ -380,7 +378,7 @@ void dq_kernel(LocalArgs a) {
       return v;
     };
     const int E = 2 * a.far + 1;
-    float* out = a.part + ((int64_t(hq) * a.n_seqs + z) * a.q_blocks + bx) * E;
+    float* out = a.part + (int64_t(hq) * a.qb.count + slot) * E;
     for (int x = tid; x < E; x += 256)
       if (x != 0 && x != E - 1) out[x] = column(kBiasPad + x);
     if (wave < 2) {
@@ -396,11 +394,11 @@ void dq_kernel(LocalArgs a) {
 }
 
 // The gradient of one head's column of the bias table, by one workgroup: the sums by distance
-// of dq_kernel's workgroups added up in order (empty ones wrote zeros), then those of each
+// of dq_kernel's workgroups added up in order (those of unused numbers wrote zeros), then those of each
 // bucket.  E distances, a thread per distance and (up to 256) stretch of the workgroups.
 __device__ __forceinline__ void bias_grad(const LocalArgs& a, int h, float* rel) {
   const int E = 2 * a.far + 1;
-  const int64_t n = int64_t(a.n_seqs) * a.q_blocks;
+  const int64_t n = a.qb.count;
   const float* const p = a.part + int64_t(h) * n * E;
   for (int x = threadIdx.x; x < E; x += 256) {
     float v[8] = {};
@@ -426,9 +424,9 @@ __device__ __forceinline__ void bias_grad(const LocalArgs& a, int h, float* rel)
   }
 }
 
-// dkv_kernel's workgroups per head and sequence.
-__host__ __device__ __forceinline__ int kv_blocks(const LocalArgs& a) {
-  return a.sink_blocks * a.sink_splits + (a.kv_blocks - a.sink_blocks) * a.splits;
+// dkv_kernel's workgroups per head.
+__host__ __device__ __forceinline__ int kv_units(const LocalArgs& a) {
+  return a.n_seqs * a.sink_blocks * a.sink_splits + a.kb.count * a.splits;
 }
 
 // 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).  The
@@ -455,24 +453,27 @@ void dkv_kernel(LocalArgs a) {
       id -= uint32_t(a.n_heads);
     }
   }
-  int wx, hk, z;
-  if (!block_of(id, kv_blocks(a), a.n_heads / a.group, a.n_seqs, wx, hk, z)) return;
+  int unit, hk;
+  if (!block_of(id, kv_units(a), a.n_heads / a.group, unit, hk)) return;
   if (POS == kPosAlibi && a.qmax != nullptr && a.group == 1 && a.n_heads <= 64)
-    by_slope(a.slopes, a.n_heads, a.n_seqs, hk, z);
-  if (z == a.n_seqs - 1) {
-    zero_tail(a, a.dk, a.dk_tok, hk * a.dk_head, wx, kv_blocks(a));
-    zero_tail(a, a.dv, a.dv_tok, hk * a.dv_head, wx, kv_blocks(a));
-  }
-  int s0, L;
-  sequence(a, z, s0, L);
+    hk = by_slope(a.slopes, a.n_heads, hk);
+  zero_tail(a, a.dk, a.dk_tok, hk * a.dk_head, unit, kv_units(a));
+  zero_tail(a, a.dv, a.dv_tok, hk * a.dv_head, unit, kv_units(a));
   // the sinks' blocks first: theirs is the longest work
-  const int n_sink = a.sink_blocks * a.sink_splits;
-  const bool sink_block = wx < n_sink;
+  const int n_sink = a.n_seqs * a.sink_blocks * a.sink_splits;
+  const bool sink_block = unit < n_sink;
   const int splits = sink_block ? a.sink_splits : a.splits;
-  const int bx = sink_block ? wx : wx - n_sink;
-  const int split = bx % splits;
-  const int k0 = (bx / splits + (sink_block ? 0 : a.sink_blocks)) * S::kOwn;
-  if (k0 >= L) return;
+  const int block = (sink_block ? unit : unit - n_sink) / splits;
+  const int split = (sink_block ? unit : unit - n_sink) % splits;
+  int z, s0, L, k0;
+  if (sink_block) {
+    z = block / a.sink_blocks;
+    sequence(a, z, s0, L);
+    k0 = block % a.sink_blocks * S::kOwn;
+    if (k0 >= L) return;
+  } else if (!find_block(a, a.kb, block, z, s0, L, k0) || k0 < a.sink_blocks * S::kOwn) {
+    return;
+  }
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -508,9 +509,9 @@ void dkv_kernel(LocalArgs a) {
     reach = 0;
     for (int g = 0; g < a.group; ++g) {
       const int h = hk * a.group + g;
-      const float2* p = a.qmax + (int64_t(h) * a.n_seqs + z) * a.q_blocks;
+      const float2* p = a.qmax + int64_t(h) * a.qb.count + a.qb.first(z, s0);
       float top[1] = {-kInf};
-      for (int i = tid; i < (L + a.q_rows - 1) / a.q_rows; i += 256)
+      for (int i = tid; i << a.qb.shift < L; i += 256)
         top[0] = __builtin_fmaxf(top[0],
                                  __builtin_fmaf(__builtin_fabsf(sc) * kn[0], p[i].x, p[i].y));
       block_max(top, red, wave, lane);
@@ -786,25 +787,33 @@ void dkv_kernel(LocalArgs a) {
     }
 }
 
-// The splits' sums of a key row added up in order.  Rows of the sinks' blocks always where they
-// are split, the others where splits > 1.  32 rows per workgroup, a thread 8 dims of dK and dV.
-__global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a) {
-  const int z = blockIdx.z, hk = blockIdx.y;
-  int s0, L;
-  sequence(a, z, s0, L);
-  const int r = blockIdx.x * 32 + (threadIdx.x >> 3);
-  const int d = 8 * (threadIdx.x & 7);
-  const int sink_rows = a.sink_blocks * (128 / a.kv_ks);
-  const bool sink = r < sink_rows;
-  const int splits = sink ? a.sink_splits : a.splits;
-  if (r >= L || splits == 1) return;
+// The splits' sums of a key row added up in order, 32 rows per workgroup, a thread 8 dims of dK
+// and dV: first the rows of the sinks' blocks, where those are split, then the others.
+__host__ __device__ __forceinline__ int join_sinks(const LocalArgs& a) {
+  return a.sink_splits > 1 ? (a.n_seqs * a.sink_blocks << a.kb.shift) / 32 : 0;
+}
+__global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a, Blocks rows) {
+  const int hk = blockIdx.y;
   const int hkv = a.n_heads / a.group;
+  const int sink_rows = a.sink_blocks << a.kb.shift;
+  const int n_sink = join_sinks(a);
+  const int d = 8 * (threadIdx.x & 7);
+  int z, s0, L, r, splits;
   const float* p;
   int64_t step;
-  if (sink) {
+  if (int(blockIdx.x) < n_sink) {
+    z = int(blockIdx.x) / (sink_rows / 32);
+    sequence(a, z, s0, L);
+    r = int(blockIdx.x) % (sink_rows / 32) * 32 + (threadIdx.x >> 3);
+    if (r >= L) return;
+    splits = a.sink_splits;
     step = int64_t(hkv) * sink_rows;
     p = a.sink_part + (int64_t(z) * splits * step + int64_t(hk) * sink_rows + r) * (2 * kHeadDim);
   } else {
+    if (!find_block(a, rows, int(blockIdx.x) - n_sink, z, s0, L, r)) return;
+    r += threadIdx.x >> 3;
+    if (r >= L || r < sink_rows) return;
+    splits = a.splits;
     step = int64_t(hkv) * a.total;
     p = a.kv_part + (int64_t(hk) * a.total + s0 + r) * (2 * kHeadDim);
   }
@@ -838,22 +847,24 @@ __global__ __launch_bounds__(256) void kv_join_kernel(LocalArgs a) {
 BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t total, int wl,
                  int wr, int ns, int far) {
   BwdPlan p;
-  const int64_t full = total / 128 + n_seqs;  // blocks of 128 rows of one head, about
+  Blocks whole;
+  whole.init(total, n_seqs, max_len, 7);
+  const int64_t full = whole.count;  // blocks of 128 rows of one head, about
   // (with a table's sums in LDS beside two KS = 2 stages a CU would hold one workgroup)
   p.ks = far > 0 ? 1 : pick_ks(full * n_heads);
-  const int q_rows = 128 / p.ks;
-  p.q_blocks = (max_len + q_rows - 1) / q_rows;
+  p.qb.init(total, n_seqs, max_len, p.ks == 2 ? 6 : 7);
   const int group = n_heads / n_kv_heads;
   p.kv_ks = pick_ks(full * n_kv_heads);
   const int kv_rows = 128 / p.kv_ks;
-  p.kv_blocks = (max_len + kv_rows - 1) / kv_rows;
+  p.kb.init(total, n_seqs, max_len, p.kv_ks == 2 ? 6 : 7);
   // steps of a workgroup that holds 64 tiles of queries at a time and KS of them per step
   const int64_t all = int64_t((max_len + kRows - 1) / kRows) * group / p.kv_ks + 1;
   const int64_t window =
       std::min<int64_t>(all, ((int64_t(wl) + wr + kv_rows) / kRows + 1) * group / p.kv_ks + 1);
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(512 / (full * n_kv_heads * p.kv_ks),
                                                         window / 6)));
-  p.sink_blocks = window < all ? std::min((ns + kv_rows - 1) / kv_rows, p.kv_blocks) : 0;
+  p.sink_blocks =
+      window < all ? (std::min(ns, max_len) + kv_rows - 1) / kv_rows : 0;
   const int64_t piece = std::max<int64_t>(6, window / p.splits);
   // (many sequences fill the GPU by themselves, and need no more than 256 MB of sums)
   const int64_t most = std::max<int64_t>(
@@ -866,8 +877,8 @@ BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t t
   p.sink_part = p.sink_splits > 1 ? int64_t(n_seqs) * p.sink_splits * n_kv_heads *
                                         p.sink_blocks * kv_rows * row
                                   : 0;
-  p.bias_part = far > 0 ? int64_t(p.q_blocks) * n_seqs * n_heads * (2 * far + 1) : 0;
-  p.norms = 2 * int64_t(p.q_blocks) * n_seqs * n_heads;
+  p.bias_part = far > 0 ? int64_t(p.qb.count) * n_heads * (2 * far + 1) : 0;
+  p.norms = 2 * int64_t(p.qb.count) * n_heads;
   return p;
 }
 
@@ -887,11 +898,11 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, bool norms, hipStream
     return hipGetLastError();
   };
   auto launch_q = [&](auto kernel, int ks) {
-    return launch(kernel, grid_blocks(a.q_blocks, a.n_heads, a.n_seqs),
+    return launch(kernel, grid_blocks(a.qb.count, a.n_heads),
                   size_t(ks == 2 ? 4 : 3) * kPairQ + extra_q);
   };
   auto launch_kv = [&](auto kernel, int ks) {
-    return launch(kernel, grid_blocks(kv_blocks(a), hkv, a.n_seqs) + (grad ? a.n_heads : 0),
+    return launch(kernel, grid_blocks(kv_units(a), hkv) + (grad ? a.n_heads : 0),
                   size_t(ks == 2 ? 4 : 3) * kPairKV + tab);
   };
   auto run = [&](auto pos, auto drop) {
@@ -920,10 +931,11 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, bool norms, hipStream
                                        : pick(std::integral_constant<int, kPosNone>{});
   if (e != hipSuccess) return e;
   if (a.splits > 1 || (a.sink_blocks > 0 && a.sink_splits > 1)) {
-    const int rows = (a.splits > 1 ? a.kv_blocks : a.sink_blocks) * (128 / a.kv_ks);
-    hipLaunchKernelGGL(kv_join_kernel,
-                       dim3(unsigned((rows + 31) / 32), unsigned(hkv), unsigned(a.n_seqs)),
-                       dim3(256), 0, st, a);
+    Blocks rows;
+    rows.init(a.total, a.n_seqs, a.max_len, 5);
+    const int blocks = join_sinks(a) + (a.splits > 1 ? rows.count : 0);
+    hipLaunchKernelGGL(kv_join_kernel, dim3(unsigned(blocks), unsigned(hkv)), dim3(256), 0, st, a,
+                       rows);
     e = hipGetLastError();
   }
   return e;

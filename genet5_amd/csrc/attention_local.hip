@@ -38,15 +38,13 @@ void local_fwd_kernel(LocalArgs a) {
   char* const ring = smem;
   float* const tab = reinterpret_cast<float*>(smem + S::kStages * kStageBytes);
 
-  int bx, hq, z;
-  if (!block_of(blockIdx.x, a.q_blocks, a.n_heads, a.n_seqs, bx, hq, z)) return;
+  int slot, hq;
+  if (!block_of(blockIdx.x, a.qb.count, a.n_heads, slot, hq)) return;
   if (POS == kPosAlibi && a.kmax != nullptr && a.n_heads <= 64)
-    by_slope(a.slopes, a.n_heads, a.n_seqs, hq, z);
-  if (z == a.n_seqs - 1) zero_tail(a, a.o, a.o_tok, hq * a.o_head, bx, a.q_blocks);
-  int s0, L;
-  sequence(a, z, s0, L);
-  const int q0 = bx * S::kOwn;
-  if (q0 >= L) return;
+    hq = by_slope(a.slopes, a.n_heads, hq);
+  zero_tail(a, a.o, a.o_tok, hq * a.o_head, slot, a.qb.count);
+  int z, s0, L, q0;
+  if (!find_block(a, a.qb, slot, z, s0, L, q0)) return;
   const int hk = hq / a.group;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -393,7 +391,7 @@ hipError_t launch_zero_behind(const LocalArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_local_fwd(const LocalArgs& a, bool wide, hipStream_t st) {
-  const dim3 grid(unsigned(grid_blocks(a.q_blocks, a.n_heads, a.n_seqs)));
+  const dim3 grid(unsigned(grid_blocks(a.qb.count, a.n_heads)));
   if (a.kmax != nullptr) {
     const hipError_t e = launch_key_norm_max(a.k, a.k_tok, a.k_head, a.total,
                                              a.n_heads / a.group, const_cast<float*>(a.kmax), st);

@@ -252,6 +252,24 @@ struct BiasChunk {
   }
 };
 
+// How blocks of 2^shift rows of the packed sequences are numbered: per > 0: that many for every
+// sequence (those past its end unused), sequence z's from z per; per = 0: sequence z's from
+// cu[z] / 2^shift + z, which leaves room for every block of the ones before, whatever their
+// lengths, and at most one number of each sequence unused.  The host, which does not know the
+// lengths, takes the one of fewer numbers: the first for sequences of about max_len.
+struct Blocks {
+  int shift, per, count;
+  __host__ __device__ void init(int64_t total, int n_seqs, int max_len, int shift_) {
+    shift = shift_;
+    per = (max_len - 1) / (1 << shift) + 1;
+    const int64_t packed = (total >> shift) + n_seqs;
+    if (int64_t(per) * n_seqs > packed) per = 0;
+    count = per > 0 ? per * n_seqs : int(packed);
+  }
+  __device__ __forceinline__ int first(int z, int s0) const {
+    return per > 0 ? z * per : (s0 >> shift) + z;
+  }
+};
 // Kernel arguments of the attention with options, forward and backward.
 struct LocalArgs {
   const uint16_t *q, *k, *v, *dout;
@@ -276,43 +294,40 @@ struct LocalArgs {
   int wl, wr, ns;                   // window (large = unlimited), first tokens always visible
   // with ALiBi, for leaving out tiles whose probabilities vanish, or nullptr: the largest key
   // norm of each 64-token block [n_kv_heads, ceil(total / 64)], and (backward) the largest
-  // query norm and the largest -lse log2(e) of each block of q_rows queries
-  // [n_heads, n_seqs, q_blocks]
+  // query norm and the largest -lse log2(e) of each block of queries [n_heads, qb.count]
   const float* kmax;
   float2* qmax;
-  int q_blocks;                     // workgroups per head and sequence, of q_rows queries
-  int q_rows;
+  Blocks qb;                        // of dq_kernel and the forward
   int ks, kv_ks;                    // Split of the kernels over queries and over keys
   // backward: the splits of a key block's query tiles (of the sinks' blocks) and their sums
-  int kv_blocks, splits, sink_blocks, sink_splits;
+  Blocks kb;
+  int splits, sink_blocks, sink_splits;
   float *kv_part, *sink_part;
   int64_t total;
   int max_len;                      // sequences are not computed past it
   DropoutParams drop;
 };
 
-// The workgroup's (x, head, sequence) of nx x heads x sequences, from a one-dimensional grid of
-// grid_blocks() workgroups, id the number of this one: consecutive workgroups go to the eight XCDs in turn, so runs of
-// kRun blocks x of one head are given to one XCD, whose L2 then serves their common tiles.
-// False: nothing to do.
+// The workgroup's (x, head) of nx x heads, from a one-dimensional grid of grid_blocks()
+// workgroups, id the number of this one: consecutive workgroups go to the eight XCDs in turn,
+// so runs of kRun blocks x of one head are given to one XCD, whose L2 then serves their common
+// tiles.  False: nothing to do.
 constexpr int kXcds = 8;
 constexpr int kRun = 8;
-__device__ __forceinline__ bool block_of(uint32_t id, int nx, int heads, int n_seqs, int& x,
-                                         int& h, int& z) {
+__device__ __forceinline__ bool block_of(uint32_t id, int nx, int heads, int& x, int& h) {
   const uint32_t j = id / kXcds;
   const uint32_t item = ((j / kRun) * kXcds + id % kXcds) * kRun + j % kRun;
-  const uint32_t pair = item / uint32_t(nx);
   x = int(item % uint32_t(nx));
-  h = int(pair % uint32_t(heads));
-  z = int(pair / uint32_t(heads));
-  return z < n_seqs;
+  h = int(item / uint32_t(nx));
+  return h < heads;
 }
-// The same in the order of falling work under ALiBi: heads by rising slope (the reach falls
-// with it), every sequence of a head before the next one's, so that the launch does not end
-// on its longest workgroups.  Up to 64 heads.
-__device__ __forceinline__ void by_slope(const float* slopes, int heads, int n_seqs, int& h,
-                                         int& z) {
-  const int pair = z * heads + h;
+inline int64_t grid_blocks(int64_t nx, int64_t heads) {
+  constexpr int64_t unit = kXcds * kRun;
+  return (nx * heads + unit - 1) / unit * unit;
+}
+// Head number r by rising ALiBi slope, so by falling work (the reach falls with the slope), so
+// that the launch does not end on its longest workgroups.  Up to 64 heads.
+__device__ __forceinline__ int by_slope(const float* slopes, int heads, int r) {
   const int lane = threadIdx.x & 63;
   const float own = lane < heads ? slopes[lane] : kInf;
   const float key = own > 0.0f ? own : 0.0f;  // no reach
@@ -321,12 +336,7 @@ __device__ __forceinline__ void by_slope(const float* slopes, int heads, int n_s
     const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(key), j));
     rank += other < key || (other == key && j < lane) ? 1 : 0;
   }
-  z = pair % n_seqs;
-  h = __builtin_ctzll(__ballot(lane < heads && rank == pair / n_seqs));
-}
-inline int64_t grid_blocks(int64_t nx, int64_t heads, int64_t n_seqs) {
-  constexpr int64_t unit = kXcds * kRun;
-  return (nx * heads * n_seqs + unit - 1) / unit * unit;
+  return __builtin_ctzll(__ballot(lane < heads && rank == r));
 }
 
 // Sequence z's first token and length, clamped to [0, total] and max_len: a malformed
@@ -335,6 +345,41 @@ __device__ __forceinline__ void sequence(const LocalArgs& a, int z, int& s0, int
   const int total = int(a.total);
   s0 = __builtin_amdgcn_readfirstlane(min(max(a.cu[z], 0), total));
   L = __builtin_amdgcn_readfirstlane(min(min(max(a.cu[z + 1], s0), total) - s0, a.max_len));
+}
+
+// Number `slot`'s sequence z, its first token s0 and length L, and the block's first row in
+// it; false where the number is unused.  Packed numbering: one load of cu_seqlens per 63
+// sequences, lane i holds sequence base + i, whose starts rise with i.  Positions clamped as by
+// sequence().
+__device__ __forceinline__ bool find_block(const LocalArgs& a, const Blocks& nb, int slot, int& z,
+                                           int& s0, int& L, int& row) {
+  const int shift = nb.shift;
+  if (nb.per > 0) {
+    z = slot / nb.per;
+    sequence(a, z, s0, L);
+    row = (slot % nb.per) << shift;
+    return row < L;
+  }
+  const int lane = threadIdx.x & 63;
+  const int total = int(a.total);
+  int base = 0;
+  for (;;) {
+    const int i = base + lane;
+    const int c = min(max(a.cu[min(i, a.n_seqs)], 0), total);
+    const bool starts = i < a.n_seqs && (c >> shift) + i <= slot;
+    const uint64_t m = __ballot(starts);
+    if ((m >> 63) != 0) {  // lane 63 is the next round's first
+      base += 63;
+      continue;
+    }
+    const int n = __builtin_popcountll(m);
+    if (n == 0) return false;  // (only a cu_seqlens that does not begin at 0)
+    z = base + n - 1;
+    s0 = __builtin_amdgcn_readlane(c, n - 1);
+    L = min(max(__builtin_amdgcn_readlane(c, n), s0) - s0, a.max_len);
+    row = (slot - (s0 >> shift) - z) << shift;
+    return row >= 0 && row < L;
+  }
 }
 
 // KS = 2: the accumulators of waves 2 and 3 added to those of waves 0 and 1, by way of LDS
@@ -404,13 +449,12 @@ __device__ __forceinline__ int alibi_reach(float top, float sl, int L) {
   return __builtin_amdgcn_readfirstlane(sl > 0.0f && w < float(L) ? max(int(w) + 1, 0) : L);
 }
 
-// Rows behind the last sequence, [cu[n_seqs], total), of one head of a bf16 tensor: zeros.
-// Called by the 256-thread workgroups x = 0 .. nx - 1 of the last sequence.
+// Rows behind the last sequence, [cu[n_seqs], total), of one head of a bf16 tensor: zeros, the
+// work of 256-thread workgroups x = 0 .. nx - 1.
 __device__ __forceinline__ void zero_tail(const LocalArgs& a, uint16_t* p, int64_t tok,
                                           int64_t head_off, int x, int nx) {
-  int s0, L;
-  sequence(a, a.n_seqs - 1, s0, L);
-  for (int64_t r = int64_t(s0) + L + int64_t(x) * 32 + (threadIdx.x >> 3); r < a.total;
+  const int end = max(a.cu[a.n_seqs], 0);
+  for (int64_t r = int64_t(end) + int64_t(x) * 32 + (threadIdx.x >> 3); r < a.total;
        r += int64_t(nx) * 32)
     *reinterpret_cast<u32x4*>(p + r * tok + head_off + 8 * (threadIdx.x & 7)) = u32x4{0, 0, 0, 0};
 }
@@ -463,8 +507,9 @@ hipError_t launch_local_bwd(const LocalArgs& a, bool wide, bool norms, hipStream
 // The splits of the key/value gradients and the floats of the backward's buffers (far: the bias
 // table's largest distance, 0 without a table).
 struct BwdPlan {
-  int ks, q_blocks;                              // of dq_kernel
-  int kv_ks, kv_blocks, splits, sink_blocks, sink_splits;  // of dkv_kernel
+  int ks, kv_ks;
+  Blocks qb, kb;
+  int splits, sink_blocks, sink_splits;
   int64_t kv_part, sink_part, bias_part, norms;
 };
 BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t total, int wl,

@@ -229,13 +229,13 @@ def test_workspace_size_counts_what_the_backward_keeps(g5lib):
 
     # 40,000 tokens keep every workgroup busy without a split
     up = lambda floats: (floats * 4 + 255) // 256 * 256
-    T, blocks = 40000, 20
+    T, blocks = 40000, 20 * 16                     # 16 sequences of 2,500: 20 blocks each
     kw = dict(total_tokens=T, max_seqlen=2500, n_seqs=16, n_heads=8, n_kv_heads=4)
-    base = 2 * up(8 * T) + up(4 * T // 64) + up(2 * blocks * 16 * 8)
+    base = 2 * up(8 * T) + up(4 * T // 64) + up(2 * blocks * 8)
     assert size(_opts(), **kw) == base
     assert size(_opts(p=0.1), **kw) == base + up(8 * T)
     assert size(_opts(bias_buckets=8, bias_distance=10), **kw) == \
-        base + up(blocks * 16 * 8 * 21)
+        base + up(blocks * 8 * 21)
     # sinks under a window: their 128 keys' tiles in pieces of the window's length
     all_steps, window = 40 * 2 + 1, ((100 + 128) // 64 + 1) * 2 + 1
     pieces = -(-all_steps // window)

@@ -428,3 +428,31 @@ def test_nothing_to_do(cuda_device):
             assert (t == 0).all()
     e = attention.flash_attn_varlen_func(q[:0], k[:0], v[:0], c, c, 0, 0, window_size=(3, 3))
     assert e.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("name", ["full_alibi", "window_sinks", "all"])
+def test_many_sequences(cuda_device, name):
+    """More sequences than lanes of a wave, empty ones among them (at both ends too), one long."""
+    case = CASES[name]
+    lens = [0, 0] + [(7 * i) % 11 for i in range(62)] + [300] + [(5 * i) % 4 for i in range(90)] + [0]
+    cu = packed(lens)
+    print(f"attention local {len(lens)} sequences {name}", flush=True)
+    q, k, v, do, tab = inputs(cu[-1] + 5, 4, 2, 61, cuda_device, table=case.get("table"))
+    res = run(q, k, v, do, cu, table=tab, **call_args(case, cuda_device))
+    want = ref.attention(q, k, v, cu, 0.125, do, table=tab, **ref_args(case))
+    compare(res, want, name, rows=cu[-1])
+    assert (res["out"][cu[-1]:] == 0).all() and (res["dk"][cu[-1]:] == 0).all()
+
+
+def test_a_cu_seqlens_that_breaks_its_contract_stays_in_bounds(cuda_device):
+    """Falling, negative and too large entries are clamped on the device: no result is promised,
+    but every access stays inside the buffers and the call ends."""
+    q, k, v, do, tab = inputs(300, 4, 2, 63, cuda_device, table=32)
+    for bad in ([0, 200, 100, 300], [0, -5, 400, 250], [50, 60, 2 ** 30, 300], [7, 7, 7, 7]):
+        c = cu_tensor(bad, cuda_device)
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v, tab)]
+        out = attention.flash_attn_varlen_func(*leaves[:3], c, c, 300, 300, window_size=(30, 30),
+                                               sink_tokens=3, relative_bias=leaves[3])
+        grads = torch.autograd.grad(out, leaves, do)
+        torch.cuda.synchronize()
+        assert out.shape == q.shape and grads[3].shape == tab.shape
