@@ -157,6 +157,7 @@ _attn_op.register_autograd(_no_backward)
 # ---- window, sinks, bucketed position bias, dropout, backward -------------------------
 
 MAX_BIAS_DISTANCE = 1024
+_INT32_MAX = 2 ** 31 - 1
 
 
 @functools.lru_cache(maxsize=64)
@@ -209,15 +210,18 @@ _BUCKETS: dict = {}
 
 
 def _buckets_on(num_buckets: int, max_distance: int, device: torch.device) -> torch.Tensor:
-    """relative_buckets on `device`, built once per device and pair of numbers."""
+    """relative_buckets on `device`, built once per device and pair of numbers and kept (a
+    captured graph may read it from then on)."""
     key = (num_buckets, max_distance, device)
     t = _BUCKETS.get(key)
     if t is None:
-        if len(_BUCKETS) >= 64:
-            _BUCKETS.clear()
-        t = _BUCKETS[key] = relative_buckets(num_buckets, max_distance, device)
-        if device.type == "cuda" and not torch.cuda.is_current_stream_capturing():
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the bucket table of a relative bias is built by the first call "
+                               "with its sizes: run one before capturing a graph")
+        t = relative_buckets(num_buckets, max_distance, device)
+        if device.type == "cuda":
             torch.cuda.current_stream(device).synchronize()  # used on any stream from now on
+        _BUCKETS[key] = t
     return t
 
 
@@ -552,7 +556,9 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
     if dropout_p and q.device.type != "cuda":
         raise NotImplementedError("attention dropout runs on the GPU only (dropout_p must be 0 "
                                   f"on {q.device})")
-    wl, wr = (int(w) for w in window_size)
+    # beyond every position is as good as unlimited
+    wl, wr, sink_tokens, max_seqlen_q = (min(int(x), _INT32_MAX) for x in
+                                         (*window_size, sink_tokens, max_seqlen_q))
     leaves = (q, k, v) if relative_bias is None else (q, k, v, relative_bias)
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in leaves)
     lse = None
@@ -586,11 +592,16 @@ _CU_CACHE: dict = {}
 
 
 def _uniform_cu_seqlens(batch: int, seqlen: int, device: torch.device) -> torch.Tensor:
-    key = (batch, seqlen, device)
+    if torch.compiler.is_compiling():
+        return torch.arange(batch + 1, dtype=torch.int32, device=device) * seqlen
+    # by stream, so that its use follows its making without a synchronisation
+    key = (batch, seqlen, device, _stream(device) if device.type == "cuda" else None)
     cu = _CU_CACHE.get(key)
     if cu is None:
-        cu = torch.arange(0, (batch + 1) * seqlen, seqlen, dtype=torch.int32, device=device)
-        _CU_CACHE.clear()
+        cu = torch.arange(batch + 1, dtype=torch.int32, device=device) * seqlen
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            return cu  # the graph's own: written by its replays only
+        # kept: a captured graph may read it from now on
         _CU_CACHE[key] = cu
     return cu
 

@@ -192,3 +192,26 @@ def test_learned_bias_reaches_the_backward_of_the_table_only(cuda_device):
         assert all((p.grad is not None) == leaf for p in x)
         tables.append(t.grad)
     assert torch.equal(*tables)
+
+
+def test_module_compiles_as_one_graph(cuda_device):
+    """The module on a [B, L, D] batch, traced without a break, training and inference."""
+    torch.manual_seed(19)
+    cfg = attention.FlashAttentionConfig(embed_dim=256, num_heads=4, num_buckets=32,
+                                         window_size=(50, 50), sink_tokens=2)
+    m = attention.FlashAttention(cfg).to(cuda_device).to(torch.bfloat16)
+    h = torch.randn(2, 120, 256, device=cuda_device).to(torch.bfloat16)
+    f = torch.compile(lambda t: m(t)[0], fullgraph=True, backend="aot_eager")
+    res = []
+    for fn in (f, lambda t: m(t)[0]):
+        m.zero_grad()
+        x = h.clone().requires_grad_(True)
+        out = fn(x)
+        out.float().pow(2).sum().backward()
+        res.append([out.detach(), x.grad] + [p.grad.clone() for p in m.parameters()])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        m.eval()
+        m._fused_projections = lambda t: False
+        assert torch.equal(f(h), m(h)[0])

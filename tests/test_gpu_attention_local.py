@@ -456,3 +456,61 @@ def test_a_cu_seqlens_that_breaks_its_contract_stays_in_bounds(cuda_device):
         grads = torch.autograd.grad(out, leaves, do)
         torch.cuda.synchronize()
         assert out.shape == q.shape and grads[3].shape == tab.shape
+
+
+def test_windows_beyond_every_position(cuda_device):
+    """Windows, sinks and lengths that pass 32 bits mean all keys."""
+    cu = [0, 200]
+    q, k, v, do, _ = inputs(200, 4, 2, 65, cuda_device)
+    want = run(q, k, v, do, cu, window_size=(1000, 1000))
+    for w in ((2 ** 31 - 1, 2 ** 31), (2 ** 32 + 5, 2 ** 40)):
+        got = run(q, k, v, do, cu, window_size=w, max_len=2 ** 33)
+        for n in want:
+            assert torch.equal(got[n], want[n]), n
+    a = run(q, k, v, do, cu, window_size=(3, 3), sink_tokens=2 ** 32)
+    for n in want:
+        ref.check(a[n], {**ref.attention(q, k, v, cu, 0.125, do)}, n) if n != "lse" else None
+
+
+def test_bucket_table_before_a_capture(cuda_device):
+    """A table that no call has built yet is refused under capture, which stays valid."""
+    q, k, v, do, tab = inputs(64, 4, 4, 67, cuda_device, table=32)
+    c = cu_tensor([0, 64], cuda_device)
+    attention._BUCKETS.pop((32, 777, q.device), None)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captur"):
+            attention.flash_attn_varlen_func(q, k, v, c, c, 64, 64, relative_bias=tab,
+                                             max_distance=777)
+        out = q * 2
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, q * 2)
+
+
+def test_fixed_length_calls_of_changing_sizes_under_graphs(cuda_device):
+    """A captured fixed-length call keeps its own sequence bounds when calls of other sizes
+    come between its replays."""
+    g = torch.Generator().manual_seed(69)
+    r = lambda B, L: torch.randn(B, L, 4, 64, generator=g).to(torch.bfloat16).to(cuda_device)
+    x = r(3, 70)
+    f = lambda t: attention.flash_attn_func(t, t, t, window_size=(20, 20))
+    with torch.no_grad():
+        want = f(x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            f(x)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f(x)
+        for rep in range(5):
+            f(r(2 + rep, 33 + rep))
+            junk = [torch.full((4,), 2 ** 30, dtype=torch.int32, device=cuda_device)
+                    for _ in range(64)]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), rep
+            del junk
