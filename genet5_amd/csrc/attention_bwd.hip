@@ -203,7 +203,9 @@ void dq_kernel(LocalArgs a) {
         const float p = __builtin_amdgcn_exp2f(t);
         float d = dp[r + e];
         if constexpr (DROP) {
-          const float mult = (e == 0 ? bits << 16 : bits) >= thr ? up : 0.0f;
+          const bool keep =
+              e == 0 ? uint16_t(bits) >= uint16_t(thr >> 16) : bits >= thr;
+          const float mult = keep ? up : 0.0f;
           d = __builtin_fmaf(d, mult, -delta);
         } else {
           d -= delta;
@@ -491,6 +493,7 @@ void dkv_kernel(LocalArgs a) {
   kr.request(a.k + int64_t(s0 + min(jk, L - 1)) * a.k_tok + hk * a.k_head, half);
   vr.request(a.v + int64_t(s0 + min(jk, L - 1)) * a.v_tok + hk * a.v_head, half);
   uint32_t thr = 0, golden_c = 0;
+  const uint32_t low = (lane & 1) ? 0 : 16;  // an even key takes the low half of a hash
   float up = 0.0f;
   if constexpr (DROP) {
     thr = min(a.drop.thr, 65535u) << 16;
@@ -622,7 +625,7 @@ void dkv_kernel(LocalArgs a) {
           const uint32_t other =
               __builtin_amdgcn_update_dpp(0u, hb[r & 7], 0xb1, 0xf, 0xf, false);  // lane ^ 1
           const uint32_t bits = (lane & 1) == (q >> 1) ? hb[r & 7] : other;
-          const float mult = ((lane & 1) ? bits : bits << 16) >= thr ? up : 0.0f;
+          const float mult = (bits << low) >= thr ? up : 0.0f;
           pd[e] = p * mult;
           d = __builtin_fmaf(d, mult, -dl4[e]);
         } else {

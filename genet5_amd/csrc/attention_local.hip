@@ -89,11 +89,18 @@ void local_fwd_kernel(LocalArgs a) {
 #pragma unroll
     for (int st = 0; st < S::kStages; ++st) issue(uint32_t(st) * kStageBytes);
   };
+  // the reference that the exponents subtract, ms: the running maximum m (0 while every term
+  // was -inf), or a fixed upper bound
+  float m = -kInf, ms = 0.0f;
+  bool fixed = false;
   if constexpr (POS != kPosAlibi) begin(L);
   qr.take(qf, iq < L, a.sc < 0.0f ? 0x80008000u : 0u);
   if constexpr (POS == kPosAlibi) {
     // With the key norms, keys farther than `reach` from every query of the workgroup are left
     // out: their terms are below 2^-40 of the query's own key's, which it sees.
+    // Where every term of the workgroup without its bias is within 32 of zero (base 2) and the
+    // bias is not positive, the upper bound |q_i| max |k| sc of a row's terms, at most 2^64
+    // above its largest, serves as its reference in place of the running maximum.
     int reach = L;
     if (a.kmax != nullptr) {
       OwnRows kr;
@@ -108,10 +115,14 @@ void local_fwd_kernel(LocalArgs a) {
           dot = __builtin_fmaf(float(qf[kc][e]), float(kf[kc][e]), dot);
       dot += __shfl_xor(dot, 32, 64);
       __shared__ float red[2][4];
-      float v[2] = {norm_max(qf), iq < L ? -sc * dot : -kInf};
+      const float qn = norm_max(qf);
+      float v[2] = {qn, iq < L ? -sc * dot : -kInf};
       block_max(v, red, wave, lane);
-      const float bound = sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
+      const float kn = key_norm(a, hk, s0, L, red, wave, lane);
+      const float bound = sc * v[0] * kn;
       reach = alibi_reach(bound + v[1], sl, L);
+      fixed = __builtin_amdgcn_readfirstlane(int(sl >= 0.0f && bound <= 32.0f)) != 0;
+      if (fixed) m = ms = sc * qn * kn;
     }
     begin(reach);
   }
@@ -132,8 +143,7 @@ void local_fwd_kernel(LocalArgs a) {
   }
 
   f32x16 o[2] = {f32x16{}, f32x16{}};
-  float m = -kInf, psum = 0.0f;
-  float ms = 0.0f;  // what the exponents subtract: m, or 0 while every term was -inf
+  float psum = 0.0f;
   f32x16 s[2];
 
   auto advance = [&](float mx) __attribute__((always_inline)) {
@@ -157,16 +167,18 @@ void local_fwd_kernel(LocalArgs a) {
   uint32_t pk[2][8];
   auto softmax = [&](auto plain_c, int n, float c) __attribute__((always_inline)) {
     constexpr bool PLAIN = decltype(plain_c)::value;
-    float mx = s[0][0];
+    if (POS != kPosAlibi || !fixed) {
+      float mx = s[0][0];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; r += 2)
-        mx = __builtin_fmaxf(__builtin_fmaxf(mx, s[b][r]), s[b][r + 1]);
-    if constexpr (PLAIN)
-      advance(POS == kPosTable ? __builtin_fmaf(mx, sc, c) : mx * sc);
-    else
-      advance(mx);
+        for (int r = 0; r < 16; r += 2)
+          mx = __builtin_fmaxf(__builtin_fmaxf(mx, s[b][r]), s[b][r + 1]);
+      if constexpr (PLAIN)
+        advance(POS == kPosTable ? __builtin_fmaf(mx, sc, c) : mx * sc);
+      else
+        advance(mx);
+    }
     const float sub = POS == kPosTable && PLAIN ? c - ms : -ms;
     const uint32_t jp = uint32_t(n * kRows + 4 * half) >> 1;
     float sum = 0.0f;
@@ -184,7 +196,7 @@ void local_fwd_kernel(LocalArgs a) {
         if constexpr (DROP) {
           const uint32_t bits =
               dropout_pair_bits(rkey, jp + uint32_t(32 * b + 8 * (r >> 2) + (r & 3)) / 2);
-          p[0] = (bits << 16) >= thr ? p[0] : 0.0f;
+          p[0] = uint16_t(bits) >= uint16_t(thr >> 16) ? p[0] : 0.0f;
           p[1] = bits >= thr ? p[1] : 0.0f;
         }
         pk[b][r >> 1] = pack_bf16x2(p[0], p[1]);
