@@ -206,11 +206,11 @@ _SIGS = {
                                   ctypes.c_int),
     "g5moe_attn_varlen_fwd": ([_P, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P,
                                ctypes.POINTER(AttnShape), _P], ctypes.c_int),
-    "g5moe_attn_local_fwd": ([_P] * 8 + [ctypes.c_float, _P, _P, _OPTS_P, _ATTN_P, _P],
+    "g5moe_attn_local_fwd": ([_P] * 8 + [ctypes.c_float, _P, _P, _P, _OPTS_P, _ATTN_P, _P],
                              ctypes.c_int),
     "g5moe_attn_bwd_workspace_size": ([_OPTS_P, _ATTN_P, ctypes.POINTER(ctypes.c_size_t)],
                                       ctypes.c_int),
-    "g5moe_attn_bwd": ([_P] * 10 + [ctypes.c_float] + [_P] * 6 +
+    "g5moe_attn_bwd": ([_P] * 11 + [ctypes.c_float] + [_P] * 6 +
                        [_OPTS_P, _ATTN_P, _ATTN_P, _P], ctypes.c_int),
     "g5moe_dropout_add": ([_P, _P, _P, _DROP_P, ctypes.c_float, ctypes.c_int64, ctypes.c_int32,
                            ctypes.c_int32, _P], ctypes.c_int),

@@ -269,12 +269,12 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                    relative_bias: Optional[torch.Tensor] = None, max_distance: int = 128,
                    window_size: Tuple[int, int] = (-1, -1), sink_tokens: int = 0,
                    dropout_p: float = 0.0, dropout_seed: int = 0, return_lse: bool = False,
-                   return_norms: bool = False):
+                   for_backward: bool = False):
     """g5moe_attn_local_fwd on the current stream: attention over the visible keys with an
     optional position bias and dropout.  Tensors as attn_varlen_fwd takes them;
-    relative_bias [num_buckets, H] bf16 or fp32.  Returns out [T, H, 64] (and softmax_lse
-    [H, T] fp32 when return_lse, and with return_norms what attn_bwd takes as key_norms);
-    rows behind the last sequence are zeros in out."""
+    relative_bias [num_buckets, H] bf16 or fp32.  Returns out [T, H, 64]; (out, softmax_lse
+    [H, T] fp32) with return_lse; with for_backward (out, softmax_lse, out_low, key_norms),
+    which attn_bwd takes.  Rows behind the last sequence are zeros in out."""
     dev = _check_device(q)
     T, H = q.shape[0], q.shape[1]
     Hkv = k.shape[1] if k.dim() == 3 else -1
@@ -291,7 +291,11 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     empty = n_seqs == 0 or max_seqlen <= 0   # nothing is launched
     out = (torch.zeros if empty else torch.empty)((T + ops.ROW_PAD, H, HEAD_DIM),
                                                   dtype=torch.bfloat16, device=dev)[:T]
-    lse = torch.empty((H, T), dtype=torch.float32, device=dev) if return_lse else None
+    lse = out_low = None
+    if return_lse or for_backward:
+        lse = torch.empty((H, T), dtype=torch.float32, device=dev)
+    if for_backward:
+        out_low = torch.empty((T, H, HEAD_DIM), dtype=torch.bfloat16, device=dev)
     shape = _lib.AttnShape(n_seqs, max_seqlen, T, H, Hkv, HEAD_DIM, 0, q.stride(0), q.stride(1),
                            k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
                            out.stride(1))
@@ -303,10 +307,10 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                          device=dev)
     ops._call_on(dev, "g5moe_attn_local_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                  _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias), _ptr(buckets),
-                 ctypes.c_float(softmax_scale), _ptr(lse), _ptr(ws), ctypes.byref(opts),
-                 ctypes.byref(shape), _stream(dev))
-    if return_norms:
-        return out, lse, ws if alibi_slopes is not None and not empty else None
+                 ctypes.c_float(softmax_scale), _ptr(lse), _ptr(out_low), _ptr(ws),
+                 ctypes.byref(opts), ctypes.byref(shape), _stream(dev))
+    if for_backward:
+        return out, lse, out_low, ws if alibi_slopes is not None and not empty else None
     return (out, lse) if return_lse else out
 
 
@@ -317,12 +321,13 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
              relative_bias: Optional[torch.Tensor] = None, max_distance: int = 128,
              window_size: Tuple[int, int] = (-1, -1), sink_tokens: int = 0,
              dropout_p: float = 0.0, dropout_seed: int = 0, bias_grad: bool = True,
-             key_norms: Optional[torch.Tensor] = None):
+             out_low: Optional[torch.Tensor] = None, key_norms: Optional[torch.Tensor] = None):
     """g5moe_attn_bwd on the current stream: (dq, dk, dv, d_relative_bias) of a forward with
     these arguments, from its out and softmax_lse; d_relative_bias is None without a table
-    or with bias_grad = False.  key_norms: the forward's (attn_local_fwd, return_norms), which
-    the call would otherwise form again under ALiBi.  Rows behind the last sequence are
-    zeros."""
+    or with bias_grad = False.  out_low: the forward's (attn_local_fwd, for_backward), what the
+    rounding of out left over, without which the gradients carry its error.  key_norms: the
+    forward's, which the call would otherwise form again under ALiBi.  Rows behind the last
+    sequence are zeros."""
     dev = _check_device(q)
     T, H = q.shape[0], q.shape[1]
     Hkv = k.shape[1] if k.dim() == 3 else -1
@@ -336,13 +341,16 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     _check_cu(cu_seqlens, dev)
     _check_position(alibi_slopes, relative_bias, max_distance, H, dev)
     ops._require(softmax_lse, "softmax_lse", (H, T), torch.float32, dev)
+    if out_low is not None:
+        ops._require(out_low, "out_low", (T, H, HEAD_DIM), torch.bfloat16, dev)
     if key_norms is not None and (
             key_norms.device != dev or key_norms.dtype != torch.uint8
             or key_norms.numel() < _lib.attn_workspace_size(T, H, Hkv, HEAD_DIM)):
         raise ValueError("key_norms must be what attn_local_fwd returned for this call")
-    return _attn_bwd(dout, q, k, v, out, softmax_lse, cu_seqlens, alibi_slopes, relative_bias,
-                     key_norms, (int(max_seqlen), softmax_scale, max_distance, *window_size,
-                                 sink_tokens, dropout_p), dropout_seed, bias_grad)
+    return _attn_bwd(dout, q, k, v, out, softmax_lse, out_low, cu_seqlens, alibi_slopes,
+                     relative_bias, key_norms, (int(max_seqlen), softmax_scale, max_distance,
+                                                *window_size, sink_tokens, dropout_p),
+                     dropout_seed, bias_grad)
 
 
 @functools.lru_cache(maxsize=256)
@@ -354,8 +362,8 @@ def _bwd_workspace_size(opts: tuple, dropout_p: float, sizes: tuple) -> int:
     return int(n.value)
 
 
-def _attn_bwd(dout, q, k, v, out, softmax_lse, cu_seqlens, alibi_slopes, relative_bias, key_norms,
-              call, dropout_seed, bias_grad):
+def _attn_bwd(dout, q, k, v, out, softmax_lse, out_low, cu_seqlens, alibi_slopes, relative_bias,
+              key_norms, call, dropout_seed, bias_grad):
     """attn_bwd on arguments that have been checked (saved by a forward)."""
     max_seqlen, softmax_scale, max_distance, wl, wr, sink_tokens, dropout_p = call
     dev = q.device
@@ -381,10 +389,10 @@ def _attn_bwd(dout, q, k, v, out, softmax_lse, cu_seqlens, alibi_slopes, relativ
         (wl, wr, sink_tokens, opts.bias_buckets, opts.bias_distance, opts.bias_dtype), dropout_p,
         sizes), dtype=torch.uint8, device=dev)
     ops._call_on(dev, "g5moe_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                 _ptr(softmax_lse), _ptr(cu_seqlens), _ptr(alibi_slopes), _ptr(bias),
-                 _ptr(buckets), ctypes.c_float(softmax_scale), _ptr(dq), _ptr(dk), _ptr(dv),
-                 _ptr(dbias), _ptr(key_norms), _ptr(ws), ctypes.byref(opts), ctypes.byref(shape),
-                 ctypes.byref(gshape), _stream(dev))
+                 _ptr(out_low), _ptr(softmax_lse), _ptr(cu_seqlens), _ptr(alibi_slopes),
+                 _ptr(bias), _ptr(buckets), ctypes.c_float(softmax_scale), _ptr(dq), _ptr(dk),
+                 _ptr(dv), _ptr(dbias), _ptr(key_norms), _ptr(ws), ctypes.byref(opts),
+                 ctypes.byref(shape), ctypes.byref(gshape), _stream(dev))
     return dq, dk, dv, dbias
 
 
@@ -393,13 +401,13 @@ def _draw_seed() -> int:
     return int(torch.randint(0, 2 ** 62, (1,)).item())
 
 
-def _bwd_call(need_bias, dout, q, k, v, out, lse, cu, slopes, bias, norms, call, seed):
+def _bwd_call(need_bias, dout, q, k, v, out, lse, low, cu, slopes, bias, norms, call, seed):
     """attn_bwd with dout brought into a form the kernel reads."""
     st = dout.stride()
     if dout.dtype != torch.bfloat16 or st[2] != 1 or st[0] % 8 or st[1] % 8 \
             or dout.data_ptr() % 16:
         dout = dout.to(torch.bfloat16).contiguous()
-    return _attn_bwd(dout, q, k, v, out, lse, cu, slopes, bias, norms, call, seed, need_bias)
+    return _attn_bwd(dout, q, k, v, out, lse, low, cu, slopes, bias, norms, call, seed, need_bias)
 
 
 class _AttnFunction(torch.autograd.Function):
@@ -409,10 +417,10 @@ class _AttnFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, cu, max_seqlen, scale, slopes, max_distance, wl, wr, sinks,
                 p, seed):
-        out, lse, norms = attn_local_fwd(q, k, v, cu, max_seqlen, scale, slopes, bias,
-                                         max_distance, (wl, wr), sinks, p, seed, return_lse=True,
-                                         return_norms=True)
-        ctx.save_for_backward(q, k, v, out, lse, cu, slopes, bias, norms)
+        out, lse, low, norms = attn_local_fwd(q, k, v, cu, max_seqlen, scale, slopes, bias,
+                                              max_distance, (wl, wr), sinks, p, seed,
+                                              for_backward=True)
+        ctx.save_for_backward(q, k, v, out, lse, low, cu, slopes, bias, norms)
         ctx.call = (max_seqlen, scale, max_distance, wl, wr, sinks, p)
         ctx.seed = seed
         ctx.mark_non_differentiable(lse)
@@ -435,46 +443,50 @@ def _attn_local_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                    max_seqlen: int, softmax_scale: float, alibi_slopes: Optional[torch.Tensor],
                    relative_bias: Optional[torch.Tensor], max_distance: int, window_left: int,
                    window_right: int, sink_tokens: int, dropout_p: float,
-                   dropout_seed: Optional[int]
-                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(out, softmax_lse [H, T], the dropout seed as host int64 [1]).  With dropout and no
-    seed the op draws one per call, so a compiled program draws anew each time."""
+                   dropout_seed: Optional[int], for_backward: bool
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(out, softmax_lse [H, T], for_backward: out_low, else an empty tensor, the dropout seed
+    as host int64 [1]).  With dropout and no seed the op draws one per call, so a compiled
+    program draws anew each time."""
     seed = 0
     if dropout_p > 0:
         seed = _draw_seed() if dropout_seed is None else dropout_seed
-    out, lse = attn_local_fwd(q, k, v, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes,
-                              relative_bias, max_distance, (window_left, window_right),
-                              sink_tokens, dropout_p, seed, return_lse=True)
-    return out, lse, torch.tensor([seed], dtype=torch.int64)
+    out, lse, *saved = attn_local_fwd(q, k, v, cu_seqlens, max_seqlen, softmax_scale,
+                                      alibi_slopes, relative_bias, max_distance,
+                                      (window_left, window_right), sink_tokens, dropout_p, seed,
+                                      return_lse=True, for_backward=for_backward)
+    low = saved[0] if for_backward else q.new_empty((0,))
+    return out, lse, low, torch.tensor([seed], dtype=torch.int64)
 
 
 @_attn_local_op.register_fake
 def _(q, k, v, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes, relative_bias, max_distance,
-      window_left, window_right, sink_tokens, dropout_p, dropout_seed):
+      window_left, window_right, sink_tokens, dropout_p, dropout_seed, for_backward):
     T, H, D = q.shape
     return (q.new_empty((T, H, D)), q.new_empty((H, T), dtype=torch.float32),
+            q.new_empty((T, H, D) if for_backward else (0,)),
             torch.empty((1,), dtype=torch.int64, device="cpu"))
 
 
 @torch.library.custom_op("g5moe::attn_local_backward", mutates_args=())
 def _attn_local_bwd_op(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                       out: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
-                       max_seqlen: int, softmax_scale: float,
+                       out: torch.Tensor, lse: torch.Tensor, out_low: torch.Tensor,
+                       cu_seqlens: torch.Tensor, max_seqlen: int, softmax_scale: float,
                        alibi_slopes: Optional[torch.Tensor],
                        relative_bias: Optional[torch.Tensor], max_distance: int,
                        window_left: int, window_right: int, sink_tokens: int, dropout_p: float,
                        seed: torch.Tensor, bias_grad: bool
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv, d_relative_bias or an empty tensor)."""
-    dq, dk, dv, db = _bwd_call(bias_grad, dout, q, k, v, out, lse, cu_seqlens, alibi_slopes,
-                               relative_bias, None, (max_seqlen, softmax_scale, max_distance,
-                                               window_left, window_right, sink_tokens,
-                                               dropout_p), int(seed[0]))
+    dq, dk, dv, db = _bwd_call(bias_grad, dout, q, k, v, out, lse, out_low, cu_seqlens,
+                               alibi_slopes, relative_bias, None,
+                               (max_seqlen, softmax_scale, max_distance, window_left,
+                                window_right, sink_tokens, dropout_p), int(seed[0]))
     return dq, dk, dv, q.new_empty((0,)) if db is None else db
 
 
 @_attn_local_bwd_op.register_fake
-def _(dout, q, k, v, out, lse, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes,
+def _(dout, q, k, v, out, lse, out_low, cu_seqlens, max_seqlen, softmax_scale, alibi_slopes,
       relative_bias, max_distance, window_left, window_right, sink_tokens, dropout_p, seed,
       bias_grad):
     grads = tuple(t.new_empty(t.shape) for t in (q, k, v))
@@ -484,23 +496,23 @@ def _(dout, q, k, v, out, lse, cu_seqlens, max_seqlen, softmax_scale, alibi_slop
 
 
 def _local_setup(ctx, inputs, output):
-    (q, k, v, cu, max_seqlen, scale, slopes, bias, max_distance, wl, wr, sinks, p, _) = inputs
-    out, lse, seed = output
-    ctx.save_for_backward(q, k, v, out, lse, cu, slopes, bias, seed)
+    (q, k, v, cu, max_seqlen, scale, slopes, bias, max_distance, wl, wr, sinks, p, _, _) = inputs
+    out, lse, low, seed = output
+    ctx.save_for_backward(q, k, v, out, lse, low, cu, slopes, bias, seed)
     ctx.call = (max_seqlen, scale, max_distance, wl, wr, sinks, p)
-    ctx.mark_non_differentiable(lse, seed)
+    ctx.mark_non_differentiable(lse, low, seed)
     ctx.set_materialize_grads(False)
 
 
-def _local_backward(ctx, dout, _dlse, _dseed):
-    grads = [None] * 14
+def _local_backward(ctx, dout, _dlse, _dlow, _dseed):
+    grads = [None] * 15
     if dout is not None:
-        q, k, v, out, lse, cu, slopes, bias, seed = ctx.saved_tensors
+        q, k, v, out, lse, low, cu, slopes, bias, seed = ctx.saved_tensors
         max_seqlen, scale, max_distance, wl, wr, sinks, p = ctx.call
         need = ctx.needs_input_grad
-        dq, dk, dv, db = _attn_local_bwd_op(dout, q, k, v, out, lse, cu, max_seqlen, scale,
-                                            slopes, bias, max_distance, wl, wr, sinks, p, seed,
-                                            need[7])
+        dq, dk, dv, db = _attn_local_bwd_op(dout, q, k, v, out, lse, low, cu, max_seqlen,
+                                            scale, slopes, bias, max_distance, wl, wr, sinks, p,
+                                            seed, need[7])
         for i, g in ((0, dq), (1, dk), (2, dv), (7, db)):
             if need[i]:
                 grads[i] = g
@@ -566,10 +578,10 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
         out, lse = _attn_op(q, k, v, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale),
                             alibi_slopes, bool(return_attn_probs))
     elif torch.compiler.is_compiling():
-        out, lse, _ = _attn_local_op(
+        out, lse, _, _ = _attn_local_op(
             q, k, v, cu_seqlens_q, int(max_seqlen_q), float(softmax_scale), alibi_slopes,
             relative_bias, int(max_distance), wl, wr, int(sink_tokens), float(dropout_p),
-            None if dropout_seed is None else int(dropout_seed))
+            None if dropout_seed is None else int(dropout_seed), grad)
     else:
         seed = 0
         if dropout_p > 0:

@@ -868,7 +868,7 @@ g5moe_status g5moe_attn_varlen_fwd(const void* q, const void* k, const void* v, 
   return hip_status(launch_attn_fwd(static_cast<const uint16_t*>(q),
                                     static_cast<const uint16_t*>(k),
                                     static_cast<const uint16_t*>(v), static_cast<uint16_t*>(out),
-                                    cu_seqlens, alibi_slopes, softmax_scale, softmax_lse,
+                                    cu_seqlens, alibi_slopes, softmax_scale, softmax_lse, nullptr,
                                     static_cast<float*>(ws), s, as_stream(stream)),
                     "g5moe_attn_varlen_fwd");
 }
@@ -948,7 +948,7 @@ static bool use_norms(const attn::LocalArgs& a) { return a.slopes != nullptr && 
 g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
                                   const int32_t* cu_seqlens, const float* alibi_slopes,
                                   const void* bias_table, const int32_t* bucket_of,
-                                  float softmax_scale, float* softmax_lse, void* ws,
+                                  float softmax_scale, float* softmax_lse, void* out_low, void* ws,
                                   const g5moe_attn_options* options,
                                   const g5moe_attn_shape* shape, void* stream) {
   G5_CHECK(check_attn_shape(shape));
@@ -963,13 +963,17 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
   G5_NONNULL(out);
   G5_NONNULL(cu_seqlens);
   const uintptr_t align = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
-                          reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out);
+                          reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out) |
+                          reinterpret_cast<uintptr_t>(out_low);
   if (align % 16 != 0)
-    return fail(G5MOE_ERR_UNSUPPORTED, "q, k, v and out must be 16-byte aligned");
+    return fail(G5MOE_ERR_UNSUPPORTED, "q, k, v, out and out_low must be 16-byte aligned");
+  if (out_low != nullptr && softmax_lse == nullptr)
+    return fail(G5MOE_ERR_INVALID_ARG, "out_low is for the backward, which needs softmax_lse too");
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
   a.o = static_cast<uint16_t*>(out);
+  a.o_low = static_cast<uint16_t*>(out_low);
   a.lse = softmax_lse;
   const bool full =
       options == nullptr || (options->window_left < 0 && options->window_right < 0);
@@ -983,8 +987,8 @@ g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, v
     g5moe_attn_shape f = s;
     f.max_seqlen = a.max_len;
     const hipError_t e = launch_attn_fwd(a.q, a.k, a.v, a.o, cu_seqlens, alibi_slopes,
-                                         softmax_scale, softmax_lse, static_cast<float*>(ws), f,
-                                         as_stream(stream));
+                                         softmax_scale, softmax_lse, a.o_low,
+                                         static_cast<float*>(ws), f, as_stream(stream));
     return hip_status(e != hipSuccess ? e : attn::launch_zero_behind(a, as_stream(stream)),
                       "g5moe_attn_local_fwd");
   }
@@ -1041,8 +1045,8 @@ g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
 }
 
 g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
-                            const void* out, const float* softmax_lse, const int32_t* cu_seqlens,
-                            const float* alibi_slopes, const void* bias_table,
+                            const void* out, const void* out_low, const float* softmax_lse,
+                            const int32_t* cu_seqlens, const float* alibi_slopes, const void* bias_table,
                             const int32_t* bucket_of, float softmax_scale, void* dq, void* dk,
                             void* dv, void* dbias, const float* key_norms, void* ws,
                             const g5moe_attn_options* options, const g5moe_attn_shape* shape,
@@ -1072,7 +1076,7 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   G5_NONNULL(dv);
   G5_NONNULL(ws);
   uintptr_t align = 0;
-  for (const void* p : {dout, q, k, v, out, static_cast<const void*>(dq),
+  for (const void* p : {dout, q, k, v, out, out_low, static_cast<const void*>(dq),
                         static_cast<const void*>(dk), static_cast<const void*>(dv)})
     align |= reinterpret_cast<uintptr_t>(p);
   if (align % 16 != 0)
@@ -1081,6 +1085,7 @@ g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, cons
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
   a.o = static_cast<uint16_t*>(const_cast<void*>(out));
+  a.o_low = static_cast<uint16_t*>(const_cast<void*>(out_low));
   a.dout = static_cast<const uint16_t*>(dout);
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);

@@ -114,6 +114,7 @@ struct AttnArgs {
   float sc;                   // softmax_scale * log2(e)
   const float* slopes;        // [n_heads] or nullptr
   float* lse;                 // [n_heads, total] (natural log) or nullptr
+  uint16_t* o_low;            // [total, n_heads, 64] contiguous: out's rounding errors, or nullptr
   const float* kmax;          // [n_kv_heads, ceil(total / 64)] largest key norm of each
                               // 64-token block, or nullptr (dense)
   int n_kblk;                 // ceil(total / 64)
@@ -569,14 +570,21 @@ void attn_fwd_kernel(AttnArgs a) {
   if (iq < L) {
     const float inv = 1.0f / l_tot;
     uint16_t* op = a.o + int64_t(s0 + iq) * a.o_tok + hq * a.o_head + 4 * half;
+    uint16_t* low = a.o_low + (int64_t(s0 + iq) * gridDim.y + hq) * 64 + 4 * half;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const float x0 = o[mb][4 * q] * inv, x1 = o[mb][4 * q + 1] * inv;
+        const float x2 = o[mb][4 * q + 2] * inv, x3 = o[mb][4 * q + 3] * inv;
         uint2 w;
-        w.x = pack_bf16x2(o[mb][4 * q] * inv, o[mb][4 * q + 1] * inv);
-        w.y = pack_bf16x2(o[mb][4 * q + 2] * inv, o[mb][4 * q + 3] * inv);
+        w.x = pack_bf16x2(x0, x1);
+        w.y = pack_bf16x2(x2, x3);
         *reinterpret_cast<uint2*>(op + 32 * mb + 8 * q) = w;
+        if (LSE && a.o_low != nullptr) {
+          const uint2 rest = {pack_rest_bf16x2(x0, x1, w.x), pack_rest_bf16x2(x2, x3, w.y)};
+          *reinterpret_cast<uint2*>(low + 32 * mb + 8 * q) = rest;
+        }
       }
     if (LSE && half == 0)
       a.lse[int64_t(hq) * a.total + s0 + iq] = (m + __builtin_log2f(l_lse)) * kLn2;
@@ -636,8 +644,8 @@ hipError_t launch_key_norm_max(const uint16_t* k, int64_t tok, int64_t head, int
 
 hipError_t launch_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* o,
                            const int32_t* cu_seqlens, const float* slopes, float softmax_scale,
-                           float* lse, float* kmax_ws, const g5moe_attn_shape& s,
-                           hipStream_t st) {
+                           float* lse, uint16_t* o_low, float* kmax_ws,
+                           const g5moe_attn_shape& s, hipStream_t st) {
   // Key-norm bounds: block skipping (with ALiBi) and the reference-max loop.  The
   // pre-pass is a launch and a read of k, 2-4 us for one sequence.  With the pass
   // against without, 12 heads, queries and keys N(0, 1), in brackets twice that (the
@@ -677,6 +685,7 @@ hipError_t launch_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t*
   a.sc = softmax_scale * kLog2e;
   a.slopes = slopes;
   a.lse = lse;
+  a.o_low = o_low;
   a.kmax = bounds ? kmax_ws : nullptr;
   a.n_kblk = n_kblk;
   a.total = s.total_tokens;

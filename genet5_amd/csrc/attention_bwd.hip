@@ -80,7 +80,7 @@ void dq_kernel(LocalArgs a) {
   const float sl = POS == kPosAlibi ? a.slopes[hq] * kLog2e : 0.0f;
 
   bf16x8 qf[4], dof[4];
-  OwnRows qr, dor, orw;
+  OwnRows qr, dor, orw, low = {};
   float lse;
   {
     const int64_t t = s0 + min(iq, L - 1);
@@ -88,6 +88,7 @@ void dq_kernel(LocalArgs a) {
     lse = a.lse[int64_t(hq) * a.total + t];
     dor.request(a.dout + t * a.do_tok + hq * a.do_head, half);
     orw.request(a.o + t * a.o_tok + hq * a.o_head, half);
+    if (a.o_low != nullptr) low.request(a.o_low + (t * a.n_heads + hq) * kHeadDim, half);
   }
   KeyTiles kt;
   TilePair<WIDE> tiles;
@@ -138,13 +139,18 @@ void dq_kernel(LocalArgs a) {
   dor.take(dof, own, 0u);
   float delta = 0.0f;
   {
-    bf16x8 of[4];
+    // The rounding of o alone would leave an error in delta that enters dS with the weight P:
+    // of a row with few keys of weight, and of the bias gradient's far buckets, which sum most
+    // of P, it would be the larger part of the error (ALiBi: dq and dk 2.6e-3 without o_low,
+    // 2.4e-3 with; the table's gradient over 2 x 4,550 tokens 3.4e-3 and 1.9e-3).
+    bf16x8 of[4], lf[4];
     orw.take(of, own, 0u);
+    low.take(lf, own, 0u);
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        delta = __builtin_fmaf(float(dof[kc][e]), float(of[kc][e]), delta);
+        delta = __builtin_fmaf(float(dof[kc][e]), float(of[kc][e]) + float(lf[kc][e]), delta);
     delta += __shfl_xor(delta, 32, 64);
   }
   uint32_t rkey = 0, thr = 0;
@@ -165,9 +171,8 @@ void dq_kernel(LocalArgs a) {
   if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
 
   f32x16 dq[2] = {f32x16{}, f32x16{}};
-  // DBIAS, per query: sums of dS and P in the far tiles (distances <= -far and >= far), and of
-  // dS in the others
-  float sum_l = 0.0f, sum_r = 0.0f, p_l = 0.0f, p_r = 0.0f, sum_near = 0.0f;
+  // DBIAS, per query: sums of dS in the far tiles (distances <= -far and >= far)
+  float sum_l = 0.0f, sum_r = 0.0f;
 
   // dS of 32 keys: half b of tile n, scores s and dP dp; c: the tile's constant bias.
   auto grad = [&](auto mask_c, auto look_c, int n, int b, const f32x16& s, const f32x16& dp,
@@ -182,7 +187,7 @@ void dq_kernel(LocalArgs a) {
     float* const dg = diag + wave * kDiagFloats;
     const uint32_t jp = uint32_t(j0) >> 1;
     const float sub = nl + c;
-    float sum = 0.0f, p_sum = 0.0f;
+    float sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       uint32_t bits = 0;
@@ -211,8 +216,7 @@ void dq_kernel(LocalArgs a) {
           d -= delta;
         }
         ds[e] = p * d;
-        if constexpr (DBIAS) sum += ds[e];
-        if constexpr (DBIAS && !LOOK) p_sum += p;
+        if constexpr (DBIAS && !LOOK) sum += ds[e];
       }
       if constexpr (DBIAS && LOOK)
         *reinterpret_cast<float2*>(dg + col * kDiagPitch + 8 * (r >> 2) + 4 * half + (r & 3)) =
@@ -235,12 +239,9 @@ void dq_kernel(LocalArgs a) {
       gtab[wave * n_tab + (n * kRows + 32 * b - wq + a.far + kBiasPad) + col - 32 * half] +=
           half == 0 ? on : all - on;
     }
-    if constexpr (DBIAS && LOOK) sum_near += sum;
     if constexpr (DBIAS && !LOOK) {
       sum_l += left ? sum : 0.0f;
       sum_r += left ? 0.0f : sum;
-      p_l += left ? p_sum : 0.0f;
-      p_r += left ? 0.0f : p_sum;
     }
   };
 
@@ -354,18 +355,7 @@ void dq_kernel(LocalArgs a) {
   if constexpr (DBIAS) {
     // the workgroup's sums by distance, clamped to +-far, in a fixed order: the tables in
     // order, then what lies past far, then the plain tiles' sums
-    // A row of dS sums to zero; what it sums to here is the error of its delta, which comes
-    // from the bf16 rounding of out.  It enters every term with the weight P, so the two end
-    // buckets, which hold most of P in long sequences, are corrected by it (2 x 4,550 tokens:
-    // relative error of the table's gradient 3.4e-3 without, 1.7e-3 with, that of its own
-    // rounding to bf16); the others hold a share of P that is too small to matter.
     __shared__ float ends[2][4];
-    {
-      const float row = sum_l + sum_r + sum_near;
-      const float err = row + __shfl_xor(row, 32, 64);
-      sum_l = __builtin_fmaf(-err, p_l, sum_l);
-      sum_r = __builtin_fmaf(-err, p_r, sum_r);
-    }
     sum_l = butterfly_sum64(sum_l);
     sum_r = butterfly_sum64(sum_r);
     if (lane == 0) {
@@ -396,8 +386,8 @@ void dq_kernel(LocalArgs a) {
 }
 
 // The gradient of one head's column of the bias table, by one workgroup: the sums by distance
-// of dq_kernel's workgroups added up in order (those of unused numbers wrote zeros), then those of each
-// bucket.  E distances, a thread per distance and (up to 256) stretch of the workgroups.
+// of dq_kernel's workgroups added up in order (those of unused numbers wrote zeros), then those
+// of each bucket.  E distances, a thread per distance and (up to 256) stretch of the workgroups.
 __device__ __forceinline__ void bias_grad(const LocalArgs& a, int h, float* rel) {
   const int E = 2 * a.far + 1;
   const int64_t n = a.qb.count;

@@ -89,18 +89,11 @@ void local_fwd_kernel(LocalArgs a) {
 #pragma unroll
     for (int st = 0; st < S::kStages; ++st) issue(uint32_t(st) * kStageBytes);
   };
-  // the reference that the exponents subtract, ms: the running maximum m (0 while every term
-  // was -inf), or a fixed upper bound
-  float m = -kInf, ms = 0.0f;
-  bool fixed = false;
   if constexpr (POS != kPosAlibi) begin(L);
   qr.take(qf, iq < L, a.sc < 0.0f ? 0x80008000u : 0u);
   if constexpr (POS == kPosAlibi) {
     // With the key norms, keys farther than `reach` from every query of the workgroup are left
     // out: their terms are below 2^-40 of the query's own key's, which it sees.
-    // Where every term of the workgroup without its bias is within 32 of zero (base 2) and the
-    // bias is not positive, the upper bound |q_i| max |k| sc of a row's terms, at most 2^64
-    // above its largest, serves as its reference in place of the running maximum.
     int reach = L;
     if (a.kmax != nullptr) {
       OwnRows kr;
@@ -115,14 +108,10 @@ void local_fwd_kernel(LocalArgs a) {
           dot = __builtin_fmaf(float(qf[kc][e]), float(kf[kc][e]), dot);
       dot += __shfl_xor(dot, 32, 64);
       __shared__ float red[2][4];
-      const float qn = norm_max(qf);
-      float v[2] = {qn, iq < L ? -sc * dot : -kInf};
+      float v[2] = {norm_max(qf), iq < L ? -sc * dot : -kInf};
       block_max(v, red, wave, lane);
-      const float kn = key_norm(a, hk, s0, L, red, wave, lane);
-      const float bound = sc * v[0] * kn;
+      const float bound = sc * v[0] * key_norm(a, hk, s0, L, red, wave, lane);
       reach = alibi_reach(bound + v[1], sl, L);
-      fixed = __builtin_amdgcn_readfirstlane(int(sl >= 0.0f && bound <= 32.0f)) != 0;
-      if (fixed) m = ms = sc * qn * kn;
     }
     begin(reach);
   }
@@ -143,7 +132,11 @@ void local_fwd_kernel(LocalArgs a) {
   }
 
   f32x16 o[2] = {f32x16{}, f32x16{}};
-  float psum = 0.0f;
+  // what the exponents subtract, ms: the running maximum m (0 while every term was -inf).  A
+  // bound of the row's terms in its place saves 3 % under ALiBi, but the probability of a row's
+  // first key is exactly 1 only against the maximum itself; else its rounding to bf16 is the
+  // larger part of a steep head's error (out 2.1e-3 against 2.3e-3, dq 2.4e-3 and 2.6e-3).
+  float m = -kInf, ms = 0.0f, psum = 0.0f;
   f32x16 s[2];
 
   auto advance = [&](float mx) __attribute__((always_inline)) {
@@ -167,18 +160,16 @@ void local_fwd_kernel(LocalArgs a) {
   uint32_t pk[2][8];
   auto softmax = [&](auto plain_c, int n, float c) __attribute__((always_inline)) {
     constexpr bool PLAIN = decltype(plain_c)::value;
-    if (POS != kPosAlibi || !fixed) {
-      float mx = s[0][0];
+    float mx = s[0][0];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2)
-          mx = __builtin_fmaxf(__builtin_fmaxf(mx, s[b][r]), s[b][r + 1]);
-      if constexpr (PLAIN)
-        advance(POS == kPosTable ? __builtin_fmaf(mx, sc, c) : mx * sc);
-      else
-        advance(mx);
-    }
+      for (int r = 0; r < 16; r += 2)
+        mx = __builtin_fmaxf(__builtin_fmaxf(mx, s[b][r]), s[b][r + 1]);
+    if constexpr (PLAIN)
+      advance(POS == kPosTable ? __builtin_fmaf(mx, sc, c) : mx * sc);
+    else
+      advance(mx);
     const float sub = POS == kPosTable && PLAIN ? c - ms : -ms;
     const uint32_t jp = uint32_t(n * kRows + 4 * half) >> 1;
     float sum = 0.0f;
@@ -239,6 +230,15 @@ void local_fwd_kernel(LocalArgs a) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) kf[b][kc] = fr.row(ring + boff + tg * kPairBytes, b, kc);
   };
+  // (behind the softmax where dropout and ALiBi take their registers)
+  constexpr bool kLateV = DROP && POS == kPosAlibi;
+  auto load_vf = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+        vf[c][mb] = fr.trans(ring + boff + tg * kPairBytes + kTileBytes, c, mb);
+  };
   auto scores = [&]() __attribute__((always_inline)) {
     const f32x16 zero16 = {};
 #pragma unroll
@@ -247,13 +247,10 @@ void local_fwd_kernel(LocalArgs a) {
       for (int b = 0; b < 2; ++b)
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][kc], qf[kc],
                                                        kc == 0 ? zero16 : s[b], 0, 0, 0);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
-        vf[c][mb] = fr.trans(ring + boff + tg * kPairBytes + kTileBytes, c, mb);
+    if constexpr (!kLateV) load_vf();
   };
   auto turn = [&]() __attribute__((always_inline)) {
+    if constexpr (kLateV) load_vf();
     // the next stage landed, and every wave has read all of this one
     gemm::wait_vmcnt<(S::kStages - 2) * 4 * KS>();
     __syncthreads();
@@ -374,14 +371,21 @@ void local_fwd_kernel(LocalArgs a) {
   if (iq < L) {
     const float inv = l == 0.0f ? 0.0f : (DROP ? a.drop.scale : 1.0f) / l;
     uint16_t* op = a.o + int64_t(s0 + iq) * a.o_tok + hq * a.o_head + 4 * half;
+    uint16_t* low = a.o_low + (int64_t(s0 + iq) * a.n_heads + hq) * kHeadDim + 4 * half;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const float x0 = o[mb][4 * q] * inv, x1 = o[mb][4 * q + 1] * inv;
+        const float x2 = o[mb][4 * q + 2] * inv, x3 = o[mb][4 * q + 3] * inv;
         uint2 w;
-        w.x = pack_bf16x2(o[mb][4 * q] * inv, o[mb][4 * q + 1] * inv);
-        w.y = pack_bf16x2(o[mb][4 * q + 2] * inv, o[mb][4 * q + 3] * inv);
+        w.x = pack_bf16x2(x0, x1);
+        w.y = pack_bf16x2(x2, x3);
         *reinterpret_cast<uint2*>(op + 32 * mb + 8 * q) = w;
+        if (a.o_low != nullptr) {
+          const uint2 rest = {pack_rest_bf16x2(x0, x1, w.x), pack_rest_bf16x2(x2, x3, w.y)};
+          *reinterpret_cast<uint2*>(low + 32 * mb + 8 * q) = rest;
+        }
       }
     if (a.lse != nullptr && half == 0)
       a.lse[int64_t(hq) * a.total + s0 + iq] = l == 0.0f ? -kInf : (m + __builtin_log2f(l)) * kLn2;

@@ -274,6 +274,7 @@ struct Blocks {
 struct LocalArgs {
   const uint16_t *q, *k, *v, *dout;
   uint16_t* o;                      // forward: written; backward: read
+  uint16_t* o_low;                  // what o's rounding left over, [total, n_heads, 64], or nullptr
   uint16_t *dq, *dk, *dv;
   const int32_t* cu;                // [n_seqs + 1]
   int64_t q_tok, k_tok, v_tok, o_tok, do_tok, dq_tok, dk_tok, dv_tok;  // element strides

@@ -223,10 +223,11 @@ hipError_t launch_pack_gate_up(const uint16_t* wg, const uint16_t* wu, uint16_t*
 hipError_t launch_pack_gate_up_t(const uint16_t* wg, const uint16_t* wu, uint16_t* wgu,
                                  uint16_t* wgu_t, const g5moe_shape& s, hipStream_t st);
 hipError_t launch_cast_f32_bf16(const float* x, uint16_t* xb, int64_t n, hipStream_t st);
+// o_low: see g5moe_attn_local_fwd; with lse only.
 hipError_t launch_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* o,
                            const int32_t* cu_seqlens, const float* slopes, float softmax_scale,
-                           float* lse, float* kmax_ws, const g5moe_attn_shape& s,
-                           hipStream_t st);
+                           float* lse, uint16_t* o_low, float* kmax_ws,
+                           const g5moe_attn_shape& s, hipStream_t st);
 
 // Rows of expert e the weight-gradient kernel reduces over: a multiple of 192
 // (three 64-row k-steps), at least 384, and at most kmax when kmax > 0.
@@ -307,6 +308,11 @@ typedef float g5_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   const g5_f32x2 v = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, g5_bf16x2));
+}
+// What that rounding left over of both values, packed alike.
+__device__ __forceinline__ uint32_t pack_rest_bf16x2(float lo, float hi, uint32_t packed) {
+  return pack_bf16x2(lo - __uint_as_float(packed << 16),
+                     hi - __uint_as_float(packed & 0xffff0000u));
 }
 
 // 16-byte global store marked non-temporal, for outputs that a later kernel

@@ -649,17 +649,20 @@ typedef struct g5moe_attn_options {
 /* Forward.  q, k, v, out, cu_seqlens, softmax_scale and shape as in g5moe_attn_varlen_fwd.
  *   alibi_slopes : fp32 [n_heads] or NULL;  bias_table : [bias_buckets, n_heads] or NULL (at
  *   most one of the two);  bucket_of : int32 [2 D + 1], each in [0, bias_buckets) (clamped);
- *   softmax_lse : fp32 [n_heads, total_tokens] out or NULL;  options : NULL = no window, no
- *   dropout;  ws : g5moe_attn_workspace_size() bytes or NULL, for the key norms with which
- *   keys whose probabilities vanish in fp32 under ALiBi are left out (each below 2^-40 of the
- *   row's largest), and which g5moe_attn_varlen_fwd (whose kernel computes long calls
- *   without any option) bounds its terms with.
- * Rows of out behind the last sequence are set to 0 (of softmax_lse, left as they were).
+ *   softmax_lse : fp32 [n_heads, total_tokens] out or NULL;  out_low : bf16 [total_tokens,
+ *   n_heads, 64] contiguous, out, for the backward, or NULL: what rounding out to bf16 left over
+ *   (with softmax_lse only);  options : NULL = no window, no dropout;
+ *   ws : g5moe_attn_workspace_size() bytes or NULL, for the key norms with which keys whose
+ *   probabilities vanish in fp32 under ALiBi are left out (each below 2^-40 of the row's
+ *   largest), and which g5moe_attn_varlen_fwd (whose kernel computes long calls without any
+ *   option) bounds its terms with.
+ * Rows of out behind the last sequence are set to 0 (of softmax_lse and out_low, left as they
+ * were).
  * Scores, softmax and sums are fp32, the probabilities enter the output product as bf16. */
 g5moe_status g5moe_attn_local_fwd(const void* q, const void* k, const void* v, void* out,
                                   const int32_t* cu_seqlens, const float* alibi_slopes,
                                   const void* bias_table, const int32_t* bucket_of,
-                                  float softmax_scale, float* softmax_lse, void* ws,
+                                  float softmax_scale, float* softmax_lse, void* out_low, void* ws,
                                   const g5moe_attn_options* options,
                                   const g5moe_attn_shape* shape, void* stream);
 
@@ -672,19 +675,22 @@ g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
 
 /* Backward of g5moe_attn_local_fwd and g5moe_attn_varlen_fwd (options NULL), from their out
  * and softmax_lse and the same inputs, options and seed.
- *   dout : bf16, the gradient of out;  dq, dk, dv : bf16 out (the gradients of key and value
- *   heads summed over the query heads that share them);  dbias : [bias_buckets, n_heads] in
- *   bias_dtype out, or NULL;  key_norms : the ws of the forward's call, which holds the key
- *   norms where ALiBi uses them, or NULL (they are formed again);
+ *   dout : bf16, the gradient of out;  out_low : the forward's, or NULL, which leaves the
+ *   rounding of out in delta = dout . out (a bias gradient of half the accuracy in long calls);
+ *   dq, dk, dv : bf16 out (the gradients of key and value heads summed over the query heads
+ *   that share them);  dbias : [bias_buckets, n_heads] in bias_dtype out, or NULL;
+ *   key_norms : the ws of the forward's call, which holds the key norms where ALiBi uses them,
+ *   or NULL (they are formed again);
  *   ws : g5moe_attn_bwd_workspace_size() bytes, 256-byte aligned;
  *   grad_shape : shape with the strides of dq, dk, dv and (its o strides) dout.
  * Rows of dq, dk and dv behind the last sequence are set to 0.  Sums are fp32; P and dS enter
  * their products as bf16.  No atomics on memory; the order of every sum is fixed. */
 g5moe_status g5moe_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
-                            const void* out, const float* softmax_lse, const int32_t* cu_seqlens,
-                            const float* alibi_slopes, const void* bias_table,
-                            const int32_t* bucket_of, float softmax_scale, void* dq, void* dk,
-                            void* dv, void* dbias, const float* key_norms, void* ws,
+                            const void* out, const void* out_low, const float* softmax_lse,
+                            const int32_t* cu_seqlens, const float* alibi_slopes,
+                            const void* bias_table, const int32_t* bucket_of,
+                            float softmax_scale, void* dq, void* dk, void* dv, void* dbias,
+                            const float* key_norms, void* ws,
                             const g5moe_attn_options* options, const g5moe_attn_shape* shape,
                             const g5moe_attn_shape* grad_shape, void* stream);
 

@@ -187,10 +187,10 @@ def test_c_refusals(g5lib, opts, shape, ptrs, scale, match):
     o, s = _opts(**opts), _shape(**shape)
     with pytest.raises(_lib.G5MoEError, match=match):
         _lib.call("g5moe_attn_local_fwd", at["q"], at["k"], at["v"], at["out"], at["cu"],
-                  at["slopes"], at["table"], at["lut"], scale, None, None, ctypes.byref(o),
+                  at["slopes"], at["table"], at["lut"], scale, None, None, None, ctypes.byref(o),
                   ctypes.byref(s), None)
     with pytest.raises(_lib.G5MoEError, match=match):
-        _lib.call("g5moe_attn_bwd", FAKE, at["q"], at["k"], at["v"], at["out"], FAKE, at["cu"],
+        _lib.call("g5moe_attn_bwd", FAKE, at["q"], at["k"], at["v"], at["out"], None, FAKE, at["cu"],
                   at["slopes"], at["table"], at["lut"], scale, FAKE, FAKE, FAKE, None, None, FAKE,
                   ctypes.byref(o), ctypes.byref(s), ctypes.byref(_shape(**shape)), None)
 
@@ -199,10 +199,16 @@ def test_c_backward_refusals(g5lib):
     o, s = _opts(), _shape()
 
     def call(dbias=None, grad=s, ws=FAKE, lse=FAKE):
-        _lib.call("g5moe_attn_bwd", FAKE, FAKE, FAKE, FAKE, FAKE, lse, FAKE, None, None, None,
+        _lib.call("g5moe_attn_bwd", FAKE, FAKE, FAKE, FAKE, FAKE, None, lse, FAKE, None, None, None,
                   0.1, FAKE, FAKE, FAKE, dbias, None, ws, ctypes.byref(o), ctypes.byref(s),
                   ctypes.byref(grad), None)
 
+    with pytest.raises(_lib.G5MoEError, match="softmax_lse"):   # out_low without it
+        _lib.call("g5moe_attn_local_fwd", FAKE, FAKE, FAKE, FAKE, FAKE, None, None, None, 0.1,
+                  None, FAKE, None, ctypes.byref(o), ctypes.byref(s), None)
+    with pytest.raises(_lib.G5MoEError, match="aligned"):
+        _lib.call("g5moe_attn_local_fwd", FAKE, FAKE, FAKE, FAKE, FAKE, None, None, None, 0.1,
+                  FAKE, FAKE + 2, None, ctypes.byref(o), ctypes.byref(s), None)
     for kw, match in ((dict(dbias=FAKE), "dbias"), (dict(grad=_shape(total_tokens=9)), "strides"),
                       (dict(ws=None), "ws is NULL"), (dict(lse=None), "softmax_lse")):
         with pytest.raises(_lib.G5MoEError, match=match):
@@ -213,8 +219,8 @@ def test_c_empty_calls_do_nothing(g5lib):
     for kw in (dict(n_seqs=0), dict(max_seqlen=0), dict(total_tokens=0)):
         s = _shape(**kw)
         _lib.call("g5moe_attn_local_fwd", None, None, None, None, None, None, None, None, 0.1,
-                  None, None, None, ctypes.byref(s), None)
-        _lib.call("g5moe_attn_bwd", None, None, None, None, None, None, None, None, None, None,
+                  None, None, None, None, ctypes.byref(s), None)
+        _lib.call("g5moe_attn_bwd", None, None, None, None, None, None, None, None, None, None, None,
                   0.1, None, None, None, None, None, None, None, ctypes.byref(s), ctypes.byref(s),
                   None)
 

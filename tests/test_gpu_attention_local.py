@@ -514,3 +514,50 @@ def test_fixed_length_calls_of_changing_sizes_under_graphs(cuda_device):
             torch.cuda.synchronize()
             assert torch.equal(out, want), rep
             del junk
+
+
+@pytest.mark.parametrize("name,L", [("full", 2100), ("full_alibi", 600), ("window_sinks", 300),
+                                    ("buckets", 77), ("dropout", 600)])
+def test_what_the_rounding_of_out_left_over(cuda_device, name, L):
+    """out_low is off out by at most half a step of bf16 (2^-8 relative), and out + out_low is
+    nearer to the 64-bit value than out (2,100 tokens without an option: the full attention's
+    kernel)."""
+    case = CASES[name]
+    cu = [0, L, L + 40]
+    print(f"attention out_low {name} {L}", flush=True)
+    q, k, v, do, tab = inputs(cu[-1], 4, 2, 21, cuda_device, table=case.get("table"))
+    kw = call_args(case, cuda_device)
+    out, lse, low, _ = attention.attn_local_fwd(
+        q, k, v, cu_tensor(cu, cuda_device), L, 0.125, kw.get("alibi_slopes"), tab,
+        kw.get("max_distance", 128), kw.get("window_size", (-1, -1)), kw.get("sink_tokens", 0),
+        kw.get("dropout_p", 0.0), kw.get("dropout_seed", 0), for_backward=True)
+    assert torch.equal(out, run(q, k, v, do, cu, grads=False, table=tab, **kw)["out"]) or \
+        name in ("full", "full_alibi")   # inference without options keeps its kernel
+    assert (low.double().abs() <= out.double().abs() * 2.0 ** -8).all()
+    want = ref.attention(q, k, v, cu, 0.125, None, table=tab, **ref_args(case))["out"]
+    a, b = (((x.double().cpu() - want).norm() / want.norm()).item()
+            for x in (out, out.double() + low.double()))
+    assert b < a, (a, b)
+
+
+@pytest.mark.parametrize("name", ["alibi", "alibi_dropout", "buckets"])
+def test_gradients_carry_two_roundings(cuda_device, name):
+    """dq and dk against the formula in 64 bits, by norm.  A value's rounding to bf16 has the
+    relative root mean square 1.66e-3: the error of a mantissa m in [1, 2) is uniform in
+    +-2^-8, its root mean square 2^-8 / sqrt 3, and the mean of 1 / m^2 is 3 / (8 ln 2) over
+    the density 1 / (m ln 2).  dS and the result are rounded: 2.35e-3; 6 % are left for the
+    probabilities' rounding in out.  With the rounding of out itself in delta it would be
+    2.6e-3."""
+    H, L = 12, 600
+    case = {"alibi": dict(slopes=attention.alibi_slopes(H)),
+            "alibi_dropout": dict(slopes=attention.alibi_slopes(H), p=0.1),
+            "buckets": dict(table=32, far=128)}[name]
+    cu = [0, L]
+    print(f"attention two roundings {name}", flush=True)
+    q, k, v, do, tab = inputs(L, H, H, 22, cuda_device, table=case.get("table"))
+    res = run(q, k, v, do, cu, table=tab, **call_args(case, cuda_device))
+    want = ref.attention(q, k, v, cu, 0.125, do, table=tab, **ref_args(case))
+    for n in ("dq", "dk"):
+        rel = ((res[n].double().cpu() - want[n]).norm() / want[n].norm()).item()
+        print(n, rel, flush=True)
+        assert rel <= 2.5e-3, (n, rel)
