@@ -6,7 +6,9 @@
 //
 // What bounds it: memory, two reads and one write (one and one in the backward) per element;
 // a thread moves 16 bytes of each operand, and its hashes (one per two elements, two for the
-// row) are hidden behind the loads.
+// row) are hidden behind the loads.  36,400 x 768 bf16: 25.7 us, backward 19 us (6.5 and 5.9
+// TB/s, where part of the operands is still in the last-level cache; a large copy reaches 4.9);
+// 777 x 768 fp32 3.2 us each, launch and latency.
 #include <algorithm>
 
 #include "g5moe_internal.h"
