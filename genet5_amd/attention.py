@@ -281,7 +281,7 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     _check_qkv(q, "q", T, H, dev)
     _check_qkv(k, "k", T, Hkv, dev)
     _check_qkv(v, "v", T, Hkv, dev)
-    if H % Hkv:
+    if Hkv < 1 or H % Hkv:
         raise ValueError(f"key/value heads {Hkv} must divide query heads {H}")
     _check_cu(cu_seqlens, dev)
     _check_position(alibi_slopes, relative_bias, max_distance, H, dev)
@@ -336,7 +336,7 @@ def attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     _check_qkv(v, "v", T, Hkv, dev)
     _check_qkv(out, "out", T, H, dev)
     _check_qkv(dout, "dout", T, H, dev)
-    if H % Hkv:
+    if Hkv < 1 or H % Hkv:
         raise ValueError(f"key/value heads {Hkv} must divide query heads {H}")
     _check_cu(cu_seqlens, dev)
     _check_position(alibi_slopes, relative_bias, max_distance, H, dev)

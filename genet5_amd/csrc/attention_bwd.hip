@@ -870,6 +870,11 @@ BwdPlan bwd_plan(int max_len, int n_seqs, int n_heads, int n_kv_heads, int64_t t
                                                         window / 6)));
   p.sink_blocks =
       window < all ? (std::min(ns, max_len) + kv_rows - 1) / kv_rows : 0;
+  // (numbered for every sequence: where most are far shorter than their sinks, and beyond what a
+  // launch holds, the sinks' blocks stay whole among the others)
+  const int64_t sinks = int64_t(n_seqs) * p.sink_blocks;
+  if (sinks > 4 * int64_t(p.kb.count) || sinks * n_kv_heads > (int64_t(1) << 22))
+    p.sink_blocks = 0;
   const int64_t piece = std::max<int64_t>(6, window / p.splits);
   // (many sequences fill the GPU by themselves, and need no more than 256 MB of sums)
   const int64_t most = std::max<int64_t>(

@@ -561,3 +561,19 @@ def test_gradients_carry_two_roundings(cuda_device, name):
         rel = ((res[n].double().cpu() - want[n]).norm() / want[n].norm()).item()
         print(n, rel, flush=True)
         assert rel <= 2.5e-3, (n, rel)
+
+
+@pytest.mark.parametrize("slopes", [None, [0.5, 0.03]])
+def test_sinks_longer_than_most_sequences(cuda_device, slopes):
+    """Many short sequences and one long one with 700 sinks: the sinks' key blocks are not
+    numbered for every sequence."""
+    lens = [i % 4 for i in range(600)] + [1500] + [3, 0, 2] * 100
+    cu = packed(lens)
+    print(f"attention sinks of many sequences {slopes}", flush=True)
+    case = dict(window=(20, 20), sinks=700)
+    if slopes:
+        case["slopes"] = slopes
+    q, k, v, do, _ = inputs(cu[-1], 2, 1, 23, cuda_device)
+    res = run(q, k, v, do, cu, **call_args(case, cuda_device))
+    want = ref.attention(q, k, v, cu, 0.125, do, **ref_args(case))
+    compare(res, want, "sinks of many sequences")
