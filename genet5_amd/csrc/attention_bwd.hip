@@ -34,7 +34,7 @@ namespace attn {
 namespace {
 
 constexpr int kPairQ = 2 * kTileBytes;         // dq_kernel: K tile, V tile
-constexpr int kVecBytes = 1024;                // dkv_kernel: -lse, delta, row keys of a tile
+constexpr int kVecBytes = 1024;                // dkv_kernel: -lse, -delta, row keys of a tile
 constexpr int kPairKV = 2 * kTileBytes + kVecBytes;
 
 // A wave adds up dS by distance in a table of its own in LDS, so the order of its sums is
@@ -179,6 +179,13 @@ void dq_kernel(LocalArgs a) {
   BiasChunk bc;
   if constexpr (POS == kPosAlibi) bc.init(sl, sc, lane);
 
+  // -delta to start the product dP from, which saves its subtraction; with dropout it follows
+  // the multiplier
+  f32x16 dp0 = {};
+  if constexpr (!DROP)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp0[r] = -delta;
+
   f32x16 dq[2] = {f32x16{}, f32x16{}};
   // DBIAS, per query: sums of dS in the far tiles (distances <= -far and >= far)
   float sum_l = 0.0f, sum_r = 0.0f;
@@ -221,8 +228,6 @@ void dq_kernel(LocalArgs a) {
               e == 0 ? uint16_t(bits) >= uint16_t(thr >> 16) : bits >= thr;
           const float mult = keep ? up : 0.0f;
           d = __builtin_fmaf(d, mult, -delta);
-        } else {
-          d -= delta;
         }
         ds[e] = p * d;
         if constexpr (DBIAS && !LOOK) sum += ds[e];
@@ -291,7 +296,7 @@ void dq_kernel(LocalArgs a) {
 #pragma unroll
         for (int kc = 0; kc < 4; ++kc)
           dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(V, b, kc), dof[kc],
-                                                       kc == 0 ? zero16 : dp, 0, 0, 0);
+                                                       kc == 0 ? dp0 : dp, 0, 0, 0);
         uint32_t pk[8];
         if constexpr (POS == kPosAlibi)
           if (!look) s = bc.add_half(s, b, float(iq - j0), before);
@@ -330,7 +335,7 @@ void dq_kernel(LocalArgs a) {
   if (own && half == 0 && tg == 0) {  // for dkv_kernel
     const int64_t at = int64_t(hq) * a.total + s0 + iq;
     a.nl[at] = nl;
-    a.delta[at] = delta;
+    a.delta[at] = -delta;
     if constexpr (DROP) a.rowkey[at] = rkey;
   }
   bool holds = true;
@@ -430,7 +435,7 @@ __host__ __device__ __forceinline__ int kv_units(const LocalArgs& a) {
   return a.n_seqs * a.sink_blocks * a.sink_splits + a.kb.count * a.splits;
 }
 
-// 32 keys per wave against the tiles of queries (Q, dO and their -lse, delta, row keys).  The
+// 32 keys per wave against the tiles of queries (Q, dO and their -lse, -delta, row keys).  The
 // tiles of a key block (of each query head that shares the key head) may be split over several
 // workgroups, `splits` of them or `sink_splits` for the blocks that hold sinks, which every
 // query sees: each writes its sums in fp32 and kv_join_kernel adds them up in order.
@@ -600,7 +605,8 @@ void dkv_kernel(LocalArgs a) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const f32x4 nl4 = *reinterpret_cast<const f32x4*>(vec + 8 * q);
-      const f32x4 dl4 = *reinterpret_cast<const f32x4*>(vec + 64 + 8 * q);
+      f32x4 dl4;
+      if constexpr (DROP) dl4 = *reinterpret_cast<const f32x4*>(vec + 64 + 8 * q);
       float pd[4], ds[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -626,10 +632,9 @@ void dkv_kernel(LocalArgs a) {
           const uint32_t bits = (lane & 1) == (q >> 1) ? hb[r & 7] : other;
           const float mult = (bits << low) >= thr ? up : 0.0f;
           pd[e] = p * mult;
-          d = __builtin_fmaf(d, mult, -dl4[e]);
+          d = __builtin_fmaf(d, mult, dl4[e]);
         } else {
           pd[e] = p;
-          d -= dl4[e];
         }
         ds[e] = p * d;
       }
@@ -690,15 +695,24 @@ void dkv_kernel(LocalArgs a) {
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          f32x16 s, dp;
+          f32x16 s, dp = zero16;
+          if constexpr (!DROP) {  // dP from -delta, as in dq_kernel
+            const float* nd = reinterpret_cast<const float*>(ring + pair + 2 * kTileBytes) + 64 +
+                              32 * b + 4 * half;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 x = *reinterpret_cast<const f32x4*>(nd + 8 * q);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dp[4 * q + e] = x[e];
+            }
+          }
 #pragma unroll
           for (int kc = 0; kc < 4; ++kc)
             s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(Q, b, kc), kf[kc],
                                                         kc == 0 ? zero16 : s, 0, 0, 0);
 #pragma unroll
           for (int kc = 0; kc < 4; ++kc)
-            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(D, b, kc), vf[kc],
-                                                         kc == 0 ? zero16 : dp, 0, 0, 0);
+            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.row(D, b, kc), vf[kc], dp, 0, 0, 0);
           uint32_t pkp[8], pkd[8];
           if constexpr (POS == kPosAlibi)
             if (!look) s = bc.add_half(s, b, float(jk - i0), before);

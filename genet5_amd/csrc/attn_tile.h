@@ -288,7 +288,7 @@ struct LocalArgs {
   int bias_bf16, n_buckets, far;
   float* lse;                       // [n_heads, total]; natural log
   float* nl;                        // backward: -lse * log2(e), [n_heads, total]
-  float* delta;                     // backward: dout . o, [n_heads, total]
+  float* delta;                     // backward: -dout . o, [n_heads, total]
   uint32_t* rowkey;                 // backward with dropout: the rows' keys, [n_heads, total]
   float* part;                      // backward: bias sums per workgroup of dq_kernel
   void* dbias;                      // backward: [n_buckets, n_heads] or nullptr
