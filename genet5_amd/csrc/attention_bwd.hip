@@ -48,8 +48,15 @@ constexpr int kGradTables = 4;
 constexpr int kDiagPitch = 34;
 constexpr int kDiagFloats = kCols * kDiagPitch;   // per wave
 
+// dq_kernel's waves per SIMD: three without a position bias, whose code fits 160 registers (12
+// heads, two against three: 8 x 4,550 tokens 818, 742 us; 2 x 4,550 230, 227; window of 256 + 256
+// over 8 x 2,048 72, 64).  ALiBi would spill three registers or subtract delta again, and its
+// launches of less than two rounds lose (8 x 4,550 366, 355; 2 x 4,550 105, 122; 4 x 1,100 35, 39);
+// the tables of the bias gradient leave LDS for two workgroups per CU.
+constexpr int dq_waves(int pos) { return pos == kPosNone ? 3 : 2; }
+
 template <int POS, bool DROP, bool DBIAS, bool WIDE, int KS>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2)))
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(dq_waves(POS), dq_waves(POS))))
 void dq_kernel(LocalArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   using S = Split<KS>;
