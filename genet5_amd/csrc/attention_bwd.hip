@@ -21,9 +21,9 @@
 // and 44 %, LDS reads 29 % without a bank conflict; 2 x 4,550 with buckets 30 and 43, 34 and
 // 37 % at 1.45 of 2 waves per SIMD (864 workgroups on 512 places).
 // Measured (dq_kernel, dkv_kernel; 12 heads; rates of the 3 and 4 products): 8 x 4,550 tokens
-// without options 810, 1,040 us (942, 978 TFLOP/s); buckets 2 x 4,550 278, 325 us (686, 782),
-// 16 x 512 56, 52 us; window of 1,024 + 1,024 over 1 x 9,000 130, 159 us; ALiBi 8 x 4,550 359,
-// 438 us.
+// without options 745, 1,060 us (1,024, 960 TFLOP/s); buckets 2 x 4,550 284, 326 us (672, 780),
+// 16 x 512 59, 53 us; window of 1,024 + 1,024 over 1 x 9,000 120, 157 us; ALiBi 8 x 4,550 360,
+// 444 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -156,9 +156,8 @@ void dq_kernel(LocalArgs a) {
   float delta = 0.0f;
   {
     // The rounding of o alone would leave an error in delta that enters dS with the weight P:
-    // of a row with few keys of weight, and of the bias gradient's far buckets, which sum most
-    // of P, it would be the larger part of the error (ALiBi: dq and dk 2.6e-3 without o_low,
-    // 2.4e-3 with; the table's gradient over 2 x 4,550 tokens 3.4e-3 and 1.9e-3).
+    // of a row with few keys of weight it would be a large part of the error (ALiBi: dq and dk
+    // 2.6e-3 without o_low, 2.4e-3 with).
     bf16x8 of[4], lf[4];
     orw.take(of, own, 0u);
     low.take(lf, own, 0u);
@@ -194,8 +193,9 @@ void dq_kernel(LocalArgs a) {
     for (int r = 0; r < 16; ++r) dp0[r] = -delta;
 
   f32x16 dq[2] = {f32x16{}, f32x16{}};
-  // DBIAS, per query: sums of dS in the far tiles (distances <= -far and >= far)
-  float sum_l = 0.0f, sum_r = 0.0f;
+  // DBIAS, per query: sums of dS and P in the far tiles (distances <= -far and >= far), and of
+  // dS in the others
+  float sum_l = 0.0f, sum_r = 0.0f, p_l = 0.0f, p_r = 0.0f, sum_near = 0.0f;
 
   // dS of 32 keys: half b of tile n, scores s and dP dp; c: the tile's constant bias.
   auto grad = [&](auto mask_c, auto look_c, int n, int b, const f32x16& s, const f32x16& dp,
@@ -210,7 +210,7 @@ void dq_kernel(LocalArgs a) {
     float* const dg = diag + wave * kDiagFloats;
     const uint32_t jp = uint32_t(j0) >> 1;
     const float sub = nl + c;
-    float sum = 0.0f;
+    float sum = 0.0f, p_sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       uint32_t bits = 0;
@@ -237,7 +237,8 @@ void dq_kernel(LocalArgs a) {
           d = __builtin_fmaf(d, mult, -delta);
         }
         ds[e] = p * d;
-        if constexpr (DBIAS && !LOOK) sum += ds[e];
+        if constexpr (DBIAS) sum += ds[e];
+        if constexpr (DBIAS && !LOOK) p_sum += p;
       }
       if constexpr (DBIAS && LOOK)
         *reinterpret_cast<float2*>(dg + col * kDiagPitch + 8 * (r >> 2) + 4 * half + (r & 3)) =
@@ -260,9 +261,12 @@ void dq_kernel(LocalArgs a) {
       gtab[wave * n_tab + (n * kRows + 32 * b - wq + a.far + kBiasPad) + col - 32 * half] +=
           half == 0 ? on : all - on;
     }
+    if constexpr (DBIAS && LOOK) sum_near += sum;
     if constexpr (DBIAS && !LOOK) {
       sum_l += left ? sum : 0.0f;
       sum_r += left ? 0.0f : sum;
+      p_l += left ? p_sum : 0.0f;
+      p_r += left ? 0.0f : p_sum;
     }
   };
 
@@ -376,7 +380,19 @@ void dq_kernel(LocalArgs a) {
   if constexpr (DBIAS) {
     // the workgroup's sums by distance, clamped to +-far, in a fixed order: the tables in
     // order, then what lies past far, then the plain tiles' sums
+    // A row of dS sums to zero; what it sums to here is the error that the rounding of the
+    // forward's probabilities leaves in delta.  It enters every term with the weight P, so the
+    // two end buckets, which hold most of P in long sequences while their own terms nearly
+    // cancel, are corrected by it (relative error of the table's gradient up to 3.4e-3 without,
+    // 1.1e-3 to 2.1e-3 with, for 7 % of dq_kernel's time at 2 x 4,550 tokens); the others hold a
+    // share of P that is too small to matter.
     __shared__ float ends[2][4];
+    {
+      const float row = sum_l + sum_r + sum_near;
+      const float err = row + __shfl_xor(row, 32, 64);
+      sum_l = __builtin_fmaf(-err, p_l, sum_l);
+      sum_r = __builtin_fmaf(-err, p_r, sum_r);
+    }
     sum_l = butterfly_sum64(sum_l);
     sum_r = butterfly_sum64(sum_r);
     if (lane == 0) {

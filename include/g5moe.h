@@ -676,7 +676,7 @@ g5moe_status g5moe_attn_bwd_workspace_size(const g5moe_attn_options* options,
 /* Backward of g5moe_attn_local_fwd and g5moe_attn_varlen_fwd (options NULL), from their out
  * and softmax_lse and the same inputs, options and seed.
  *   dout : bf16, the gradient of out;  out_low : the forward's, or NULL, which leaves the
- *   rounding of out in delta = dout . out (a bias gradient of half the accuracy in long calls);
+ *   rounding of out in delta = dout . out (relative errors of dq and dk up to 10 % larger);
  *   dq, dk, dv : bf16 out (the gradients of key and value heads summed over the query heads
  *   that share them);  dbias : [bias_buckets, n_heads] in bias_dtype out, or NULL;
  *   key_norms : the ws of the forward's call, which holds the key norms where ALiBi uses them,

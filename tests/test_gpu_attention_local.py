@@ -577,3 +577,20 @@ def test_sinks_longer_than_most_sequences(cuda_device, slopes):
     res = run(q, k, v, do, cu, **call_args(case, cuda_device))
     want = ref.attention(q, k, v, cu, 0.125, do, **ref_args(case))
     compare(res, want, "sinks of many sequences")
+
+
+@pytest.mark.parametrize("buckets,far,p,lens", [(8, 20, 0.25, (1500, 1100)), (16, 64, 0.0, (2300,)),
+                                                (32, 128, 0.0, (700, 900))])
+def test_bias_gradient_where_one_bucket_holds_most(cuda_device, buckets, far, p, lens):
+    """The end buckets hold most of a row's probability, and their terms nearly cancel, so an
+    error of delta shows there: by norm at most half more than the result's own rounding to
+    bf16 (1.66e-3)."""
+    case = dict(table=buckets, far=far, **(dict(p=p) if p else {}))
+    cu = packed(lens)
+    print(f"attention bias gradient {buckets} {far} {lens}", flush=True)
+    q, k, v, do, tab = inputs(cu[-1], 4, 2, 24, cuda_device, table=buckets)
+    res = run(q, k, v, do, cu, table=tab, **call_args(case, cuda_device))
+    want = ref.attention(q, k, v, cu, 0.125, do, table=tab, **ref_args(case))["dtable"]
+    rel = ((res["dtable"].double().cpu() - want).norm() / want.norm()).item()
+    print("dtable", rel, flush=True)
+    assert rel <= 2.5e-3
