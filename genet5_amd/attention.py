@@ -301,7 +301,7 @@ def attn_local_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                            out.stride(1))
     opts = _options(*window_size, sink_tokens, dropout_p, dropout_seed, bias, max_distance)
     ws = None
-    if bias is None and (alibi_slopes is not None or dropout_p == 0):
+    if alibi_slopes is not None or (bias is None and dropout_p == 0 and max(window_size) < 0):
         # for the key norms: ALiBi's reach, the bounds of long calls without any option
         ws = torch.empty(_lib.attn_workspace_size(T, H, Hkv, HEAD_DIM), dtype=torch.uint8,
                          device=dev)
@@ -428,7 +428,7 @@ class _AttnFunction(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops._once_differentiable
     def backward(ctx, dout, _dlse):
         none = (None,) * 14
         if dout is None:

@@ -44,7 +44,7 @@ class _DropoutAdd(torch.autograd.Function):
         return _launch("g5moe_dropout_add", x, residual, p, alpha, seed)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops._once_differentiable
     def backward(ctx, dout):
         if dout is None:
             return None, None, None, None, None

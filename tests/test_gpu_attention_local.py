@@ -594,3 +594,37 @@ def test_bias_gradient_where_one_bucket_holds_most(cuda_device, buckets, far, p,
     rel = ((res["dtable"].double().cpu() - want).norm() / want.norm()).item()
     print("dtable", rel, flush=True)
     assert rel <= 2.5e-3
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    q, k, v, do, _ = inputs(70, 4, 2, 25, cuda_device)
+    q = q.requires_grad_()
+    c = cu_tensor([0, 70], cuda_device)
+    out = attention.flash_attn_varlen_func(q, k, v, c, c, 70, 70)
+    plain = torch.autograd.grad(out, q, do, retain_graph=True)[0]
+    dq = torch.autograd.grad(out, q, do, create_graph=True)[0]
+    assert torch.equal(plain, dq)
+    with pytest.raises(RuntimeError):  # dq has no graph: nothing else of it required a gradient
+        torch.autograd.grad(dq.float().sum(), q)
+
+
+@pytest.mark.parametrize("name", ["window_sinks", "dropout_alibi", "buckets"])
+def test_saved_tensors_that_come_back_with_other_strides(cuda_device, name):
+    """Hooks that keep saved tensors elsewhere give back contiguous copies of strided views."""
+    case = CASES[name]
+    cu = [0, 150, 380]
+    print(f"attention saved tensors {name}", flush=True)
+    _, _, _, do, tab = inputs(cu[-1], 4, 4, 26, cuda_device, table=case.get("table"))
+    qkv = inputs(cu[-1], 12, 12, 27, cuda_device)[0].requires_grad_()
+    c = cu_tensor(cu, cuda_device)
+
+    def grad():
+        q, k, v = qkv[:, :4], qkv[:, 4:8], qkv[:, 8:]
+        out = attention.flash_attn_varlen_func(q, k, v, c, c, 230, 230, relative_bias=tab,
+                                               **call_args(case, cuda_device))
+        return torch.autograd.grad(out, qkv, do)[0]
+
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        got = grad()
+    assert torch.equal(got, want)

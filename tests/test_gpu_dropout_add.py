@@ -132,3 +132,12 @@ def test_graph_replays(cuda_device):
         for g, w in zip(res, want[rep % 3]):
             assert torch.equal(g, w)
         step(*sets[(rep + 1) % 3])
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    x = torch.randn(5, 64, device=cuda_device, requires_grad=True)
+    do = torch.randn(5, 64, device=cuda_device, requires_grad=True)
+    out = residual.dropout_add(x, torch.zeros_like(x), 0.5, seed=3)
+    dx = torch.autograd.grad(out, x, do, create_graph=True)[0]
+    with pytest.raises(RuntimeError):  # (torch names do as unused)
+        torch.autograd.grad(dx.sum(), do)
