@@ -17,9 +17,9 @@
 // forward: a value's rounding is 2^-8 relative, of random sign, and the sums average over it.
 //
 // What bounds it: matrix and vector instructions together.  Counters, all SIMDs, 8 x 4,550
-// tokens, 12 heads, ALiBi: dq_kernel matrix units busy 37 %, vector issue 49 %; dkv_kernel 40
-// and 44 %, LDS reads 29 % without a bank conflict; 2 x 4,550 with buckets 30 and 43, 34 and
-// 37 % at 1.45 of 2 waves per SIMD (864 workgroups on 512 places).
+// tokens, 12 heads, ALiBi: dq_kernel matrix units busy 38 %, vector issue 44 %; dkv_kernel 40
+// and 39 %, LDS reads 29 % without a bank conflict; 2 x 4,550 with buckets 30 and 45, 34 and
+// 33 % at 1.45 of 2 waves per SIMD (864 workgroups on 512 places).
 // Measured (dq_kernel, dkv_kernel; 12 heads; rates of the 3 and 4 products): 8 x 4,550 tokens
 // without options 745, 1,060 us (1,024, 960 TFLOP/s); buckets 2 x 4,550 284, 326 us (672, 780),
 // 16 x 512 59, 53 us; window of 1,024 + 1,024 over 1 x 9,000 120, 157 us; ALiBi 8 x 4,550 360,
